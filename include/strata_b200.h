@@ -191,6 +191,135 @@ int32_t strata_b200_embed_bf16(const int32_t *ids, int64_t rows,
 int32_t strata_b200_argmax_bf16(const uint16_t *x, int64_t rows, int64_t cols,
                                 int32_t *out, void *stream);
 
+/* ------------------------------------------------------------------------ */
+/* Several continuations of a sequence: drafted trees and beams             */
+/* ------------------------------------------------------------------------ */
+/* No counterpart in the reference.  Shared conventions:
+ *  - Caches are contiguous [batch, kv_heads, max_len, head_dim] when
+ *    block_table is null, else page pools [num_pages, kv_heads, page_size,
+ *    head_dim] with a block table I32 [batch, max_len / page_size] (page_size a
+ *    power of two from 16 to 4096); batch (or pool) * kv_heads * positions is
+ *    below 2^31.
+ *  - A workspace is device memory of at least the bytes its *_workspace_bytes
+ *    function gives (0 for a shape the entry point refuses), 16-byte aligned,
+ *    whose contents do not matter before or after a call.  Two calls that may
+ *    overlap on the GPU need two workspaces; so do two CUDA graphs that may be
+ *    replayed at once.
+ *  - `status` (null, or one I32 on the device) is set when a device-side
+ *    input is wrong, and left alone otherwise: 2 a length, position or index
+ *    out of range, 6 a block-table entry that names no page of the pool.
+ *  - Calls allocate nothing and may be captured into a CUDA graph.  Launches
+ *    go to the current device, which must be the stream's. */
+
+/* Attention of a tree of drafted tokens over the cached prompt.  q
+ * [batch * tokens, heads * head_dim]; k_new, v_new [batch * tokens,
+ * kv_heads * head_dim].  Sequence b has base[b] cached positions and count[b]
+ * live nodes (null: `tokens` for all).  Node i's k and v are written at position
+ * base + i, and node t attends to the positions below base and to the live
+ * nodes j whose bit j % 32 of word j / 32 is set in mask [batch, tokens,
+ * ceil(tokens / 32)] row t (set a node's own bit to let it see itself).  out
+ * [batch * tokens, heads * head_dim]; a node that sees nothing, and rows at or
+ * past count, are zeros.  A sequence with base < 0, count outside 0..tokens or
+ * base + count > max_len gets status 2: zeros, and nothing is appended.
+ * Positions on missing pages get status 6 and read as zero rows.  tokens <=
+ * 1024, head_dim 64 or 128, at most 128 query heads per kv head, pointers
+ * 16-byte aligned.  Two sequences must not append to the same page. */
+uint64_t strata_b200_tree_attention_workspace_bytes(int64_t tokens,
+                                                    int64_t heads,
+                                                    int64_t kv_heads,
+                                                    int64_t head_dim);
+int32_t strata_b200_tree_attention_bf16(
+    const uint16_t *q, const uint16_t *k_new, const uint16_t *v_new,
+    uint16_t *k_cache, uint16_t *v_cache, const int32_t *block_table,
+    const int32_t *base, const int32_t *count, const uint32_t *mask,
+    int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
+    int64_t head_dim, int64_t max_len, int64_t page_size, int64_t num_pages,
+    void *workspace, uint16_t *out, int32_t *status, void *stream);
+
+/* A beam step's selection.  logits [batch * beams, vocab]; scores
+ * [batch * beams], the beams' accumulated log probabilities (-inf or NaN: an
+ * empty beam); done [batch * beams] (may be null), non-zero for a beam that has
+ * ended.  A live beam w offers score + log_softmax(logits)[v] for every v (a NaN
+ * logit counts as -inf); an ended one offers its unchanged score with token
+ * eos.  Writes the `keep` best of every batch entry, best first, ties to the
+ * lowest w * vocab + v: out_scores, out_parent (the row b * beams + w),
+ * out_token and out_done (the parent had ended, or the token is eos), each
+ * [batch, keep].  Where no candidate above -inf is left: -inf, -1, -1, 0.
+ * eos -1: no token ends a beam (an ended beam's token is then -1).  keep <=
+ * 64, beams <= 1024, batch * beams <= 65535, vocab <= 2^30.  Scores are added
+ * and compared in f64 and rounded once; the softmax's terms are f32. */
+uint64_t strata_b200_beam_select_workspace_bytes(int64_t batch, int64_t beams,
+                                                 int64_t vocab, int64_t keep);
+int32_t strata_b200_beam_select_bf16(
+    const uint16_t *logits, const float *scores, const int32_t *done,
+    int64_t batch, int64_t beams, int64_t vocab, int64_t keep, int64_t eos,
+    float *out_scores, int32_t *out_parent, int32_t *out_token,
+    int32_t *out_done, void *workspace, void *stream);
+int32_t strata_b200_beam_select_f32(
+    const float *logits, const float *scores, const int32_t *done,
+    int64_t batch, int64_t beams, int64_t vocab, int64_t keep, int64_t eos,
+    float *out_scores, int32_t *out_parent, int32_t *out_token,
+    int32_t *out_done, void *workspace, void *stream);
+
+/* Keeps the accepted branch of a drafted tree: in each of n_caches caches or
+ * pools (a host array of device pointers, at most 256, 16-byte aligned; rows
+ * of row_bytes bytes, a multiple of 16), row base[b] + path[b, i] moves to
+ * base[b] + i for i < n_path[b].  path [batch, max_path] is strictly increasing
+ * from 0 or more; a sequence whose path is not, or leaves max_len, is left
+ * alone (status 2; 6 for a missing page).  max_path <= 1024.  The rows from
+ * base on must belong to the sequence alone. */
+int32_t strata_b200_kv_accept(
+    void *const *caches, int64_t n_caches, int64_t row_bytes,
+    const int32_t *block_table, const int32_t *base, const int32_t *path,
+    const int32_t *n_path, int64_t batch, int64_t kv_heads, int64_t max_len,
+    int64_t max_path, int64_t page_size, int64_t num_pages, int32_t *status,
+    void *stream);
+
+/* Gives every row of a block table a new parent: row r continues old row
+ * parents[r] (-1: becomes empty) with its length.  Pools are page pools as
+ * above with rows of row_bytes bytes, at most 256; refs [num_pages] counts who
+ * holds a page (every table entry >= 0 is one reference; more may be held
+ * elsewhere).  Full pages are shared.  A partly filled last page stays with
+ * the lowest row that takes it when nobody else holds it; every other row gets
+ * a copy of its filled rows in a free page, in every pool.  Then each
+ * non-empty row gets free pages until len + reserve positions fit; entries
+ * past those are -1 (pages an old row held beyond its length are let go).
+ * Pages no entry names any more and nobody else holds become free (refs 0);
+ * free pages are dealt out lowest id first, to rows in ascending order.
+ * Outputs: table_out [rows, pages_per_seq], lens_out, refs_out (none may be its
+ * input) and report I32 [4]: error, pages copied, pages newly reserved, pages
+ * left free.  Errors: 2 a parent or length out of range (or len + reserve past
+ * the row), 3 refs below the table's references, 5 too few free pages (report
+ * [3] is how many more are needed), 6 a needed entry that names no page; the
+ * outputs are then copies of the inputs and the pools are not touched.
+ * rows <= 65536. */
+uint64_t strata_b200_kv_fork_workspace_bytes(int64_t rows,
+                                             int64_t pages_per_seq,
+                                             int64_t num_pages);
+int32_t strata_b200_kv_fork(
+    void *const *pools, int64_t n_pools, int64_t row_bytes, int64_t kv_heads,
+    int64_t page_size, int64_t num_pages, const int32_t *table_in,
+    const int32_t *lens_in, const int32_t *refs_in, const int32_t *parents,
+    int64_t rows, int64_t pages_per_seq, int64_t reserve, int32_t *table_out,
+    int32_t *lens_out, int32_t *refs_out, int32_t *report, void *workspace,
+    void *stream);
+
+/* Moves the used pages (refs > 0) of the pools together: of n used pages, the
+ * i-th with an id of n or more moves to the i-th free id below n.  Outputs:
+ * table_out, refs_out (neither may be its input), remap [num_pages] (a page's
+ * new id, -1 for a free page; for other holders of page ids) and report I32
+ * [4]: error, used pages, pages moved, free pages.  Errors: 3 a negative count
+ * or a table entry on a page without references, 6 an entry past the pool;
+ * the outputs are then copies of the inputs (remap the identity) and the pools
+ * are not touched.  The same pool arguments as kv_fork. */
+uint64_t strata_b200_kv_compact_workspace_bytes(int64_t num_pages);
+int32_t strata_b200_kv_compact(
+    void *const *pools, int64_t n_pools, int64_t row_bytes, int64_t kv_heads,
+    int64_t page_size, int64_t num_pages, const int32_t *table_in,
+    const int32_t *refs_in, int64_t rows, int64_t pages_per_seq,
+    int32_t *table_out, int32_t *refs_out, int32_t *remap, int32_t *report,
+    void *workspace, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
