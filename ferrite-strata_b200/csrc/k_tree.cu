@@ -1,100 +1,923 @@
-// Attention of a tree of drafted tokens over a cached prompt.
+// Attention of a tree of drafted tokens over a cached prompt, on the
+// 5th-generation tensor cores (tcgen05, TMEM, TMA): bf16, head_dim 64 or 128.
 //
 // Sequence b has base[b] cached positions and count[b] live nodes.  Node i's k
 // and v rows are appended at position base + i, and node t attends to every
-// position below base and to the nodes whose bit is set in its mask row.  A
-// node at or past count, and one that sees nothing, gives zeros.
+// position below base and to the nodes whose bit is set in its mask row:
+//   o[t, h] = sum_p softmax_p(q[t, h] . k[p] / sqrt d) v[p]
+// A node at or past count, and one that sees nothing, gives zeros.
+//
+// Work.  The query rows of one (sequence, kv head) are its nodes times the
+// group's heads (row = node * G + head), so a kv head's cache is read once for
+// all of them.  An item is 128 such rows (up to 256 when there are more than
+// 128), and its KV is a list of 128-position tiles: the cached positions, read
+// from the cache or its pages, then the nodes, read from k_new and v_new
+// directly (so nothing waits for the append, which the softmax warps do while
+// the first tiles are on their way).  All tiles of all items are numbered in
+// one line and each block takes an equal run of it, whatever the sequences'
+// lengths; an item cut by a block's end leaves (max, sum, O) of each part in
+// the workspace and a second kernel joins the parts in order, so results do not
+// depend on timing.  What bounds it: reading the cache (HBM) up to about 128
+// rows a kv head, the softmax between the two products beyond.
+//
+// Block.  Warp 0 loads by TMA through one ring of 128-row tiles in the order
+// they are used (K0, K1, V0, K2, V1, ...); warp 1 issues the products
+//   S = Q K^T    (A, B in shared memory; 128 x 128 f32 in TMEM)
+//   O += P V     (A = P in TMEM, written over S; B = the V tile as loaded)
+// and warps 2-5 and 6-9 are two softmax groups, one thread per query row.  With
+// more than 128 rows the two groups take a query tile each and share every KV
+// tile; with up to 128 rows both work for the same query tile, one on the even
+// and one on the odd KV tiles (each with a maximum, sum and O of its own, joined
+// at the end), so that one group's softmax runs during the other's products.
+//
+// Softmax in base 2: O is rescaled in TMEM only when a row's maximum grows by
+// more than 8, so probabilities stay below 2^8; P is rounded to bf16 for the
+// second product, maximum, sum and O are f32.
+//
+// Masked places.  A masked score becomes -inf whatever it was.  0 * NaN must
+// not reach O either: V rows at or past a tile's end are zeroed in shared
+// memory, and so are non-finite values of a node's v; the rows that do see
+// such a node get its non-finite values added to their output.
+//
+// Every wait is bounded; one that runs out sets error word 4 and the block
+// winds down (loads land, products finish, TMEM is freed).
+#include <algorithm>
+
 #include "common.cuh"
 #include "k_branch.cuh"
+#include "k_tc.cuh"
 
 namespace sb {
 
 namespace {
 
-struct TreeSeq {
-  int base, count;  // count 0 where the sequence is unusable
-  bool bad;
+using namespace tc;
+
+constexpr int kTile = 128;  // query rows per tile, positions per KV tile
+constexpr int kThreads = 320;
+constexpr uint32_t kTmemCols = 512;  // S_0, S_1 (128 columns each), O_0, O_1 (head_dim each)
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kRescale = 8.0f;  // log2 of the largest P before O is rescaled
+
+// Shared memory: two query tiles (both of an item, or one of this segment and
+// one of the next), the ring, the second group's statistics, the barriers.
+template <int D>
+struct Lay {
+  static constexpr int kKB = D / 64;             // 64-wide blocks of head_dim
+  static constexpr int kBytesTile = 128 * D * 2;  // kKB blocks of [128 rows][128 bytes]
+  static constexpr int kSlots = D == 128 ? 5 : 8;
+  static constexpr int kQ = 0;
+  static constexpr int kRing = 2 * kBytesTile;
+  static constexpr int kStat = kRing + kSlots * kBytesTile;  // float2 [128]
+  static constexpr int kBar = kStat + 1024;
+  static constexpr int kBars = 2 * kSlots + 14;
+  static constexpr int kBytes = kBar + kBars * 8 + 16 + 1024;
+  static constexpr uint32_t kOCol = 256;
+  static_assert(kBytes <= 232448, "shared memory");
+  // One part of a cut item and query tile: O as [D / 4][128 rows] float4, then (max, sum) [128 rows].
+  static constexpr size_t kPart = size_t(D / 4) * 128 * 16 + 128 * 8;
 };
 
-__device__ __forceinline__ TreeSeq tree_seq(const int32_t* base, const int32_t* count, int tokens, int max_len, int b) {
-  TreeSeq s{base[b], count ? count[b] : tokens, false};
-  if (s.count < 0 || s.count > tokens || s.base < 0 || s.base > max_len - s.count) {
-    s.count = 0;
-    s.bad = true;
-  }
+// What the joining kernel needs to know of the item a block's run starts in.
+struct Meta {
+  int b, kvh, pair;
+  int j0;  // the item's tile the run starts at (0: the run starts with the item)
+  int nt;  // tiles of the item
+  int chunk, pad[2];
+};
+
+struct Args {
+  const int32_t *base, *count;
+  const uint32_t* mask;
+  const uint16_t *k_new, *v_new;
+  uint16_t *k_cache, *v_cache, *out;
+  int batch, tokens, heads, kv_heads, max_len;
+  int group, tpt;  // query heads per kv head; nodes per query tile (tpt * group <= 128)
+  int words;       // mask words per node
+  KvPages kp;
+  int pool_rows;
+  Meta* meta;
+  uint8_t* parts;
+  int* err;
+};
+
+struct Seq {
+  int base, count;  // count 0 where the sequence is unusable or has no nodes
+  int prefix;       // tiles of cached positions
+  int nt;           // all tiles
+  int pairs;        // items per kv head
+};
+
+__device__ __forceinline__ Seq seq_of(const Args& a, int b, int per_item, bool* bad = nullptr) {
+  Seq s;
+  s.base = a.base[b];
+  s.count = a.count ? a.count[b] : a.tokens;
+  const bool wrong = s.count < 0 || s.count > a.tokens || s.base < 0 || s.base > a.max_len - s.count;
+  if (bad) *bad = wrong;
+  if (wrong) s.base = s.count = 0;
+  s.prefix = (s.base + kTile - 1) / kTile;
+  s.nt = s.count ? s.prefix + (s.count + kTile - 1) / kTile : 0;
+  s.pairs = (s.count + per_item - 1) / per_item;
   return s;
 }
 
-__global__ void tree_append_kernel(const TreeArgs a) {
-  const int b = int(blockIdx.y), t = int(blockIdx.x);
-  const TreeSeq s = tree_seq(a.base, a.count, int(a.tokens), int(a.max_len), b);
-  if (s.bad && threadIdx.x == 0 && a.err) atomicExch(a.err, kBadPosition);
-  const int d = int(a.head_dim), w = int(a.kv_heads) * d;
-  const int64_t r = int64_t(b) * a.tokens + t;
-  if (t >= s.count) {
-    for (int i = threadIdx.x; i < int(a.heads) * d; i += blockDim.x) a.out[r * a.heads * d + i] = 0;
-    return;
+// A block's stretch of one item: tiles [j0, j1) of nt.
+struct Seg {
+  Seq s;
+  int b, kvh, pair, j0, j1;
+};
+
+// Walks the segments of a block's run.
+struct Walk {
+  int b, left;
+  int64_t off;  // within sequence b's tiles
+};
+
+__device__ __forceinline__ bool next_seg(const Args& a, int per_item, Walk& w, Seg& g) {
+  if (w.left <= 0) return false;
+  for (;;) {
+    if (w.b >= a.batch) return false;
+    g.s = seq_of(a, w.b, per_item);
+    const int64_t units = int64_t(g.s.nt) * a.kv_heads * g.s.pairs;
+    if (w.off < units) break;
+    w.off -= units;  // zero: runs end where sequences do
+    ++w.b;
   }
-  for (int i = threadIdx.x; i < w; i += blockDim.x) {
-    const int64_t row = kv_row(a.kp, b, i / d, int(a.kv_heads), int(a.max_len), s.base + t);
-    if (row < 0) {
-      if (a.err) atomicExch(a.err, kBadPage);
+  g.b = w.b;
+  const int item = int(w.off / g.s.nt);
+  g.j0 = int(w.off % g.s.nt);
+  g.kvh = item / g.s.pairs;
+  g.pair = item % g.s.pairs;
+  g.j1 = min(g.s.nt, g.j0 + w.left);
+  w.left -= g.j1 - g.j0;
+  w.off += g.j1 - g.j0;
+  return true;
+}
+
+// Tile j of a segment: valid positions, and for a tile of nodes the first node (-1 for cached positions).
+__device__ __forceinline__ int tile_valid(const Seq& s, int j, int& node0) {
+  if (j < s.prefix) {
+    node0 = -1;
+    return min(kTile, s.base - j * kTile);
+  }
+  node0 = (j - s.prefix) * kTile;
+  return min(kTile, s.count - node0);
+}
+
+// 2^x by the hardware approximation (relative error about 2^-22).
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float fmax3(float a, float b, float c) {
+  float m;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+  return m;
+}
+// Packed pairs of f32.
+__device__ __forceinline__ uint64_t pack_f2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack_f2(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma_f2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// Both halves of a bf16 pair: the non-finite ones set to zero (keep = false) or all others (keep = true).
+__device__ __forceinline__ uint32_t split_finite(uint32_t v, bool keep) {
+  const bool lo = (v & 0x7F80u) == 0x7F80u, hi = (v & 0x7F800000u) == 0x7F800000u;
+  return (lo == keep ? v & 0xFFFFu : 0u) | (hi == keep ? v & 0xFFFF0000u : 0u);
+}
+
+// Appends the block's share of the new rows, and zeroes the output rows of
+// dead nodes.  Threads 0..255 (the softmax groups').
+template <int D>
+__device__ void append_rows(const Args& a, int tid) {
+  constexpr int kPer = D / 8;  // 16-byte pieces per head
+  const int rows = a.batch * a.tokens, pieces = a.kv_heads * kPer;
+  for (int r = int(blockIdx.x); r < rows; r += int(gridDim.x)) {
+    const int b = r / a.tokens, t = r % a.tokens;
+    bool bad;
+    const Seq s = seq_of(a, b, 1, &bad);
+    if (bad && t == 0 && tid == 0 && a.err) atomicExch(a.err, kBadPosition);
+    if (t >= s.count) {
+      uint4* o = reinterpret_cast<uint4*>(a.out) + int64_t(r) * a.heads * kPer;
+      for (int i = tid; i < a.heads * kPer; i += 256) o[i] = make_uint4(0, 0, 0, 0);
       continue;
     }
-    a.k_cache[row * d + i % d] = a.k_new[r * w + i];
-    a.v_cache[row * d + i % d] = a.v_new[r * w + i];
+    const uint4* kn = reinterpret_cast<const uint4*>(a.k_new) + int64_t(r) * pieces;
+    const uint4* vn = reinterpret_cast<const uint4*>(a.v_new) + int64_t(r) * pieces;
+    for (int i = tid; i < pieces; i += 256) {
+      const int64_t row = kv_row(a.kp, b, i / kPer, a.kv_heads, a.max_len, s.base + t);
+      if (row < 0) {
+        if (a.err) atomicExch(a.err, kBadPage);
+        continue;
+      }
+      const uint4 k = kn[i], v = vn[i];
+      reinterpret_cast<uint4*>(a.k_cache)[row * kPer + i % kPer] = k;
+      reinterpret_cast<uint4*>(a.v_cache)[row * kPer + i % kPer] = v;
+    }
   }
 }
 
-// One warp per (node, head): each position's product is summed over the lanes,
-// with a running maximum and sum.
-__global__ void tree_warp_kernel(const TreeArgs a) {
-  const int b = int(blockIdx.z), h = int(blockIdx.y) * int(blockDim.y) + int(threadIdx.y), t = int(blockIdx.x);
-  const int lane = threadIdx.x, d = int(a.head_dim), per = d / 32;
-  const TreeSeq s = tree_seq(a.base, a.count, int(a.tokens), int(a.max_len), b);
-  if (h >= a.heads || t >= s.count) return;
-  const int kvh = h / int(a.heads / a.kv_heads);
-  const int64_t r = int64_t(b) * a.tokens + t;
-  const uint32_t* mask = a.mask + r * ((a.tokens + 31) / 32);
-  float q[4], o[4] = {0, 0, 0, 0}, m = -INFINITY, l = 0.0f;
-  for (int e = 0; e < per; ++e) q[e] = bf2f(a.q[(r * a.heads + h) * d + lane * per + e]) * rsqrtf(float(d));
-  for (int p = 0; p < s.base + s.count; ++p) {
-    const int j = p - s.base;
-    if (j >= 0 && !(mask[j / 32] >> (j % 32) & 1)) continue;
-    const int64_t row = kv_row(a.kp, b, kvh, int(a.kv_heads), int(a.max_len), p);
-    if (row < 0) {
-      if (a.err) atomicExch(a.err, kBadPage);
-      continue;
+template <int D, bool Wide>
+__global__ void __launch_bounds__(kThreads, 1)
+    tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                          const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap knmap,
+                          const __grid_constant__ CUtensorMap vnmap, const Args a) {
+  using L = Lay<D>;
+  constexpr int kNS = L::kSlots;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBar);
+  uint64_t* full = bars;                // [kNS] ring slot loaded
+  uint64_t* empty = bars + kNS;         // [kNS] ring slot read by its products
+  uint64_t* q_full = bars + 2 * kNS;    // [2]
+  uint64_t* q_empty = q_full + 2;       // [2]
+  uint64_t* s_full = q_full + 4;        // [2] per group: S is in TMEM
+  uint64_t* p_full = q_full + 6;        // [2] per group: P is in TMEM (4 warps arrive)
+  uint64_t* o_done = q_full + 8;        // [2] per group: the segment's last P V is complete
+  uint64_t* st_full = q_full + 10;      // the second group's statistics are written (4 warps)
+  uint64_t* o1_free = q_full + 11;      // the first group has read O_1 and the statistics (4 warps)
+  uint64_t* mma_done = q_full + 12;     // every product of the block is complete
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + L::kBars);
+  float2* stat = reinterpret_cast<float2*>(smem + L::kStat);
+  __shared__ int s_fail;
+  __shared__ int s_odd[4];  // s_odd[i % 4] == i + 1: segment i holds non-finite node values
+  __shared__ Walk s_walk;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int per_item = a.tpt * (Wide ? 2 : 1);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kNS; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
     }
-    float x = 0.0f;
-    for (int e = 0; e < per; ++e) x += q[e] * bf2f(a.k_cache[row * d + lane * per + e]);
-    x = warp_sum(x);
-    const float mn = fmaxf(m, x), c = m == -INFINITY ? 0.0f : expf(m - mn), w = expf(x - mn);
-    l = l * c + w;
-    for (int e = 0; e < per; ++e) o[e] = o[e] * c + w * bf2f(a.v_cache[row * d + lane * per + e]);
-    m = mn;
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&q_full[s], 1);
+      mbar_init(&q_empty[s], 1);
+      mbar_init(&s_full[s], 1);
+      mbar_init(&p_full[s], 4);
+      mbar_init(&o_done[s], 1);
+    }
+    mbar_init(st_full, 4);
+    mbar_init(o1_free, 4);
+    mbar_init(mma_done, 1);
+    s_fail = 0;
+    s_odd[0] = s_odd[1] = s_odd[2] = s_odd[3] = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    prefetch_map(&qmap);
+    prefetch_map(&kmap);
+    prefetch_map(&vmap);
+    prefetch_map(&knmap);
+    prefetch_map(&vnmap);
   }
-  for (int e = 0; e < per; ++e)
-    a.out[(r * a.heads + h) * d + lane * per + e] = f2bf(l > 0.0f || l != l ? o[e] / l : 0.0f);
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(tmem_slot)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  pdl_trigger();
+  pdl_wait();  // every operand may come from the kernels before
+  if (warp == 0) {
+    // All tiles in one line; this block's run starts in sequence b at tile off.
+    int64_t total = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += 32) {
+      int64_t u = 0;
+      if (b0 + lane < a.batch) {
+        const Seq s = seq_of(a, b0 + lane, per_item);
+        u = int64_t(s.nt) * a.kv_heads * s.pairs;
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
+      total += u;
+    }
+    const int64_t chunk = (total + gridDim.x - 1) / gridDim.x;
+    const int64_t w0 = chunk * blockIdx.x;
+    Walk w{a.batch, 0, 0};
+    if (w0 < total) {
+      int64_t before = 0;
+      for (int b0 = 0; b0 < a.batch; b0 += 32) {
+        int64_t u = 0;
+        if (b0 + lane < a.batch) {
+          const Seq s = seq_of(a, b0 + lane, per_item);
+          u = int64_t(s.nt) * a.kv_heads * s.pairs;
+        }
+        int64_t end = u;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int64_t y = __shfl_up_sync(0xffffffffu, end, o);
+          if (lane >= o) end += y;
+        }
+        end += before;
+        const uint32_t hit = __ballot_sync(0xffffffffu, w0 < end);
+        if (hit) {
+          const int l = __ffs(hit) - 1;
+          w.b = b0 + l;
+          w.off = w0 - (__shfl_sync(0xffffffffu, end, l) - __shfl_sync(0xffffffffu, u, l));
+          break;
+        }
+        before = __shfl_sync(0xffffffffu, end, 31);
+      }
+      w.left = int(min(chunk, total - w0));
+    }
+    if (lane == 0) {
+      s_walk = w;
+      Meta m{0, 0, 0, 0, 0, int(chunk), {0, 0}};
+      Walk w2 = w;
+      Seg g;
+      if (next_seg(a, per_item, w2, g)) {
+        m.b = g.b;
+        m.kvh = g.kvh;
+        m.pair = g.pair;
+        m.j0 = g.j0;
+        m.nt = g.s.nt;
+      }
+      a.meta[blockIdx.x] = m;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  auto fail = [&]() { atomicExch(&s_fail, 1); };
+  auto failed = [&]() { return *reinterpret_cast<volatile int*>(&s_fail) != 0; };
+
+  // Every role walks the same segments and counts ring loads, S tiles and
+  // segments for itself, so each barrier's phase is known without any
+  // block-wide synchronisation.  Ring loads of a segment of n tiles that
+  // starts at load c0:  K_0: c0;  K_j: c0 + 2j - 1;  V_j: c0 + 2j + 2, the last one c0 + 2n - 1.
+  Walk walk = s_walk;
+  Seg g;
+  if (warp == 0) {
+    // ---- TMA -------------------------------------------------------------------
+    int nl = 0, si = 0;
+    bool ok = true;
+    const int br = a.kp.paged() ? min(a.kp.page_size, kTile) : kTile;  // rows per box
+    const int nbox = kTile / br;
+    while (ok && next_seg(a, per_item, walk, g)) {
+      if (__any_sync(0xffffffffu, failed())) break;
+      const int qb = Wide ? 0 : si & 1, use = Wide ? si : si >> 1;
+      if (lane == 0) {
+        if (use >= 1 && !mbar_wait(&q_empty[qb], (use - 1) & 1)) ok = false;
+        if (ok) {
+          const int t0 = g.pair * per_item;
+          const bool second = Wide && t0 + a.tpt < g.s.count;
+          const uint32_t bytes = uint32_t(L::kKB * a.tpt * a.group * 128);
+          mbar_expect_tx(&q_full[qb], second ? 2 * bytes : bytes);
+          for (int t = 0; t < (second ? 2 : 1); ++t)
+            for (int kb = 0; kb < L::kKB; ++kb)
+              tma_load_3d(smem + L::kQ + (Wide ? t : qb) * L::kBytesTile + kb * 16384, &qmap, &q_full[qb], kb * 64,
+                          g.kvh * a.group, g.b * a.tokens + t0 + t * a.tpt);
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      if (!ok) break;
+      // This lane's box of tile j: the map row of its first position.  A page
+      // that is missing is read past the map's end, which gives zeros.
+      auto box_row = [&](int j) {
+        if (j >= g.s.prefix || lane >= nbox) return 0;
+        const int p = j * kTile + lane * br;
+        if (!a.kp.paged()) return (g.b * a.kv_heads + g.kvh) * a.max_len + p;
+        const int64_t row = p < a.max_len ? kv_row(a.kp, g.b, g.kvh, a.kv_heads, a.max_len, p) : -1;
+        if (row < 0 && p < g.s.base && a.err) atomicExch(a.err, kBadPage);
+        return row < 0 ? a.pool_rows : int(row);
+      };
+      auto load = [&](int j, int row, bool is_v) {
+        const int slot = nl % kNS, round = nl / kNS;
+        if (lane == 0) {
+          if (round >= 1 && !mbar_wait(&empty[slot], (round - 1) & 1)) ok = false;
+          if (ok) mbar_expect_tx(&full[slot], L::kBytesTile);
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (!ok) return;
+        uint8_t* dst = smem + L::kRing + slot * L::kBytesTile;
+        if (j < g.s.prefix) {
+          if (lane < nbox)
+            for (int kb = 0; kb < L::kKB; ++kb)
+              tma_load_2d(dst + kb * 16384 + lane * br * 128, is_v ? &vmap : &kmap, &full[slot], kb * 64, row);
+        } else if (lane == 0) {
+          for (int kb = 0; kb < L::kKB; ++kb)
+            tma_load_2d(dst + kb * 16384, is_v ? &vnmap : &knmap, &full[slot], g.kvh * D + kb * 64,
+                        g.b * a.tokens + (j - g.s.prefix) * kTile);
+        }
+        ++nl;
+      };
+      int row = box_row(g.j0);
+      load(g.j0, row, false);
+      for (int j = g.j0; j < g.j1 && ok; ++j) {
+        const int row1 = j + 1 < g.j1 ? box_row(j + 1) : 0;
+        if (j + 1 < g.j1) load(j + 1, row1, false);
+        if (ok) load(j, row, true);
+        row = row1;
+      }
+      ++si;
+    }
+    if (!ok) fail();
+    // Let the loads in flight land before the block can end.
+    if (lane == 0) {
+      for (int c = max(0, nl - kNS); c < nl; ++c) mbar_wait(&full[c % kNS], (c / kNS) & 1);
+      for (int s = max(0, si - (Wide ? 1 : 2)); s < si; ++s)
+        mbar_wait(&q_full[Wide ? 0 : s & 1], (Wide ? s : s >> 1) & 1);
+    }
+  } else if (warp == 1) {
+    // ---- products (lane 0 issues; the warp waits and cleans V) -------------------
+    constexpr uint32_t kIdS = idesc_bf16(kTile, kTile), kIdO = idesc_bf16(kTile, D, true);
+    int c0 = 0, si = 0;
+    int np[2] = {0, 0};  // P tiles of each group so far
+    bool ok = true;
+    auto wait_load = [&](int c) { return mbar_wait_warp(&full[c % kNS], (c / kNS) & 1); };
+    auto slot_of = [&](int c) { return smem + L::kRing + (c % kNS) * L::kBytesTile; };
+    auto release = [&](int c) {
+      if (lane == 0) umma_commit(&empty[c % kNS]);
+      __syncwarp();
+    };
+    auto issue_s = [&](int t, const uint8_t* q, const uint8_t* k) {
+      tc_fence_after();
+      if (lane == 0) {
+#pragma unroll
+        for (int kb = 0; kb < L::kKB; ++kb) {
+          const uint64_t da = sw128_desc(q + kb * 16384), db = sw128_desc(k + kb * 16384);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            umma_bf16(tmem + uint32_t(t * 128), da + uint64_t(2 * kk), db + uint64_t(2 * kk), kIdS, (kb | kk) != 0);
+        }
+        umma_commit(&s_full[t]);
+      }
+      __syncwarp();
+    };
+    while (ok && next_seg(a, per_item, walk, g)) {
+      if (__any_sync(0xffffffffu, failed())) break;
+      const int n = g.j1 - g.j0;
+      const int qb = Wide ? 0 : si & 1, use = Wide ? si : si >> 1;
+      const bool second = Wide ? g.pair * per_item + a.tpt < g.s.count : n > 1;  // the second group has work
+      const uint8_t* q0 = smem + L::kQ + qb * L::kBytesTile;
+      auto k_load = [&](int i) { return i == 0 ? c0 : c0 + 2 * i - 1; };
+      auto v_load = [&](int i) { return i == n - 1 ? c0 + 2 * n - 1 : c0 + 2 * i + 2; };
+      auto release_q = [&]() {
+        if (lane == 0) umma_commit(&q_empty[qb]);
+        __syncwarp();
+      };
+      if (!(ok = mbar_wait_warp(&q_full[qb], use & 1) && wait_load(k_load(0)))) break;
+      issue_s(0, q0, slot_of(k_load(0)));
+      if constexpr (Wide) {
+        if (second) issue_s(1, q0 + L::kBytesTile, slot_of(k_load(0)));
+        release(k_load(0));
+        if (n == 1) release_q();
+      } else {
+        release(k_load(0));
+        if (second) {
+          if (!(ok = wait_load(k_load(1)))) break;
+          issue_s(1, q0, slot_of(k_load(1)));
+          release(k_load(1));
+        }
+        if (n <= 2) release_q();
+      }
+      for (int i = 0; i < n && ok; ++i) {
+        uint8_t* v = slot_of(v_load(i));
+        if (!(ok = wait_load(v_load(i)))) break;
+        int node0;
+        const int nv = tile_valid(g.s, g.j0 + i, node0), nv16 = (nv + 15) & ~15;
+        bool dirty = false;
+        // Rows past the tile's end, up to the last 16-row step of the product.
+        for (int e = lane; e < (nv16 - nv) * L::kKB * 8; e += 32) {
+          const int piece = e & 7, kb = (e >> 3) % L::kKB, r = nv + (e >> 3) / L::kKB;
+          *reinterpret_cast<uint4*>(v + kb * 16384 + r * 128 + piece * 16) = make_uint4(0, 0, 0, 0);
+          dirty = true;
+        }
+        if (node0 >= 0) {
+          bool odd = false;
+          for (int e = lane; e < nv * L::kKB * 8; e += 32) {  // the swizzle only permutes a row's pieces
+            const int piece = e & 7, kb = (e >> 3) % L::kKB, r = (e >> 3) / L::kKB;
+            uint4* p = reinterpret_cast<uint4*>(v + kb * 16384 + r * 128 + piece * 16);
+            const uint4 x = *p;
+            const uint4 y = make_uint4(split_finite(x.x, false), split_finite(x.y, false), split_finite(x.z, false),
+                                       split_finite(x.w, false));
+            if (x.x != y.x || x.y != y.y || x.z != y.z || x.w != y.w) {
+              *p = y;
+              odd = true;
+            }
+          }
+          if (__any_sync(0xffffffffu, odd)) {
+            dirty = true;
+            if (lane == 0) {
+              *reinterpret_cast<volatile int*>(&s_odd[si & 3]) = si + 1;
+              __threadfence_block();
+            }
+          }
+        }
+        if (__any_sync(0xffffffffu, dirty)) {
+          fence_proxy_async();
+          __syncwarp();
+        }
+        const uint64_t vd = sw128_desc_mn(v, 16384);
+        auto issue_o = [&](int t, bool first, bool last) {
+          tc_fence_after();
+          if (lane == 0) {
+            const uint32_t tP = tmem + uint32_t(t * 128), tO = tmem + L::kOCol + uint32_t(t * D);
+            for (int kk = 0; kk < nv16 / 16; ++kk)
+              umma_bf16_ts(tO, tP + uint32_t(kk * 8), vd + uint64_t(kk * (2048 >> 4)), kIdO, !(first && kk == 0));
+            if (last) umma_commit(&o_done[t]);
+          }
+          __syncwarp();
+        };
+        if constexpr (Wide) {
+          if (i + 1 < n && !(ok = wait_load(k_load(i + 1)))) break;
+          for (int t = 0; t < (second ? 2 : 1) && ok; ++t) {
+            if (!(ok = mbar_wait_warp(&p_full[t], np[t] & 1))) break;
+            ++np[t];
+            issue_o(t, i == 0, i == n - 1);
+            if (i + 1 < n) issue_s(t, q0 + t * L::kBytesTile, slot_of(k_load(i + 1)));
+          }
+          if (!ok) break;
+          release(v_load(i));
+          if (i + 1 < n) release(k_load(i + 1));
+          if (i == n - 2) release_q();
+        } else {
+          const int t = i & 1;
+          if (!(ok = mbar_wait_warp(&p_full[t], np[t] & 1))) break;
+          ++np[t];
+          issue_o(t, i < 2, i + 2 >= n);
+          release(v_load(i));
+          if (i + 2 < n) {
+            if (!(ok = wait_load(k_load(i + 2)))) break;
+            issue_s(t, q0, slot_of(k_load(i + 2)));
+            release(k_load(i + 2));
+            if (i + 3 == n) release_q();
+          }
+        }
+      }
+      if (!ok) break;
+      c0 += 2 * n;
+      ++si;
+    }
+    if (!ok) fail();
+    if (lane == 0) umma_commit(mma_done);
+    __syncwarp();
+    mbar_wait_warp(mma_done, 0);
+  } else {
+    // ---- softmax and output: thread = query row ------------------------------------
+    append_rows<D>(a, int(threadIdx.x) - 64);
+    const int t = (warp - 2) >> 2;  // group
+    const int quarter = warp & 3, row = quarter * 32 + lane;
+    const uint32_t lane_addr = uint32_t(quarter * 32) << 16;
+    const uint32_t tS = tmem + lane_addr + uint32_t(t * 128);
+    const uint32_t tO = tmem + lane_addr + L::kOCol;
+    const float sl = kLog2e / sqrtf(float(D));
+    const int node = row / a.group, head = row % a.group;
+    int ns = 0, si = 0, no[2] = {0, 0};  // S tiles, segments and finished O's so far
+    while (next_seg(a, per_item, walk, g)) {
+      if (__any_sync(0xffffffffu, failed())) break;
+      const int n = g.j1 - g.j0;
+      const int tok = g.pair * per_item + (Wide ? t * a.tpt : 0) + node;  // this row's node
+      const bool live = node < a.tpt && tok < g.s.count;
+      const bool warp_live = __any_sync(0xffffffffu, live);
+      const bool mine = !Wide || t == 0 || g.pair * per_item + a.tpt < g.s.count;
+      const int64_t qrow = int64_t(g.b) * a.tokens + tok;
+      float m_ref = -INFINITY, l = 0.0f;
+      bool ok = true;
+      if (mine) {
+        // The loop stays converged: a lane whose wait ran out stops waiting and
+        // records the failure; no output is written then.
+        for (int i = Wide ? 0 : t; i < n; i += Wide ? 1 : 2) {
+          int node0;
+          const int nv = tile_valid(g.s, g.j0 + i, node0);
+          uint32_t seen[4] = {0, 0, 0, 0};
+          if (node0 >= 0 && live) {
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+              if (node0 / 32 + w < a.words) seen[w] = a.mask[qrow * a.words + node0 / 32 + w];
+          }
+          if (ok && !mbar_wait(&s_full[t], ns & 1)) ok = false;
+          ++ns;
+          __syncwarp();  // the poll may have split the warp; tcgen05.ld needs it whole
+          tc_fence_after();
+          if (warp_live) {
+            uint32_t r[kTile];
+            tmem_ld64(tS, r);
+            tmem_ld64(tS + 64, r + 64);
+            if (node0 >= 0) {
+#pragma unroll
+              for (int e = 0; e < kTile; ++e)
+                if (!(seen[e / 32] >> (e % 32) & 1) || e >= nv) r[e] = 0xFF800000u;
+            } else if (nv < kTile) {
+#pragma unroll
+              for (int e = 0; e < kTile; ++e)
+                if (e >= nv) r[e] = 0xFF800000u;
+            }
+            // Row maximum of the raw scores, four independent chains; the scale is
+            // positive, so it is applied once to the maximum (base 2).
+            float mc[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int e = 0; e < kTile; e += 8)
+#pragma unroll
+              for (int c = 0; c < 4; ++c)
+                mc[c] = fmax3(mc[c], __uint_as_float(r[e + 2 * c]), __uint_as_float(r[e + 2 * c + 1]));
+            const float mt = fmaxf(fmaxf(mc[0], mc[1]), fmaxf(mc[2], mc[3])) * sl;
+            bool rescale = false;
+            float corr = 1.0f;
+            if (mt > m_ref + kRescale) {  // also the first tile with anything to see (m_ref = -inf)
+              if (m_ref != -INFINITY) {
+                corr = ex2(m_ref - mt);
+                rescale = true;
+              }
+              l *= corr;
+              m_ref = mt;
+            }
+            // P = 2^(s sl - m_ref) as bf16 pairs, packed in place; -inf gives 0 (a row
+            // that sees nothing yet uses 0 for the maximum: no inf - inf).  bf16 by
+            // integer rounding: P is not negative, and this keeps the conversion off the
+            // pipe that computes the exponentials.
+            const float mneg = m_ref == -INFINITY ? 0.0f : -m_ref;
+            const uint64_t sl2 = pack_f2(sl, sl), mneg2 = pack_f2(mneg, mneg);
+            uint64_t acc[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int e = 0; e < kTile; e += 2) {
+              float x0, x1;
+              unpack_f2(fma_f2(pack_f2(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), sl2, mneg2), x0, x1);
+              x0 = ex2(x0);
+              x1 = ex2(x1);
+              acc[(e >> 1) & 3] = add_f2(acc[(e >> 1) & 3], pack_f2(x0, x1));
+              r[e / 2] = __byte_perm(__float_as_uint(x0) + 0x8000u, __float_as_uint(x1) + 0x8000u, 0x7632);
+            }
+            float a0, a1, a2, a3;
+            unpack_f2(add_f2(acc[0], acc[1]), a0, a1);
+            unpack_f2(add_f2(acc[2], acc[3]), a2, a3);
+            l += (a0 + a1) + (a2 + a3);
+            // O is settled: its last P V completed before this S was published.
+            if (__any_sync(0xffffffffu, rescale)) {
+#pragma unroll
+              for (int c = 0; c < D / 32; ++c) {
+                uint32_t o32[32];
+                tmem_ld32(tO + uint32_t(t * D + c * 32), o32);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o32[e] = __float_as_uint(__uint_as_float(o32[e]) * corr);
+                tmem_st32(tO + uint32_t(t * D + c * 32), o32);
+              }
+            }
+            tmem_st64(tS, r);
+          }
+          tc_fence_before();
+          __syncwarp();
+          // The first group reads O_1 of the segment before; until it has, the
+          // next P V must not start.
+          if (!Wide && t == 1 && i == 1 && si >= 1 && ok && !mbar_wait(o1_free, (si - 1) & 1)) ok = false;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[t]);
+        }
+      }
+      if (!Wide && t == 1) {
+        if (n < 2 && si >= 1 && ok && !mbar_wait(o1_free, (si - 1) & 1)) ok = false;
+        stat[row] = make_float2(m_ref, l);
+        if (!__all_sync(0xffffffffu, ok)) {
+          fail();
+          break;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(st_full);
+        ++si;
+        continue;
+      }
+      if (mine) {
+        if (ok && !mbar_wait(&o_done[t], no[t] & 1)) ok = false;
+        ++no[t];
+      }
+      float w0 = 1.0f, w1 = 0.0f;  // weights of O_0 and O_1 (the first group joins both)
+      if (!Wide) {
+        if (n > 1) {
+          if (ok && !mbar_wait(&o_done[1], no[1] & 1)) ok = false;
+          ++no[1];
+        }
+        if (ok && !mbar_wait(st_full, si & 1)) ok = false;
+        __syncwarp();
+        if (n > 1) {
+          const float2 other = stat[row];
+          const float m = fmaxf(m_ref, other.x);
+          if (m != -INFINITY) {
+            w0 = ex2(m_ref - m);
+            w1 = ex2(other.x - m);
+          }
+          l = l * w0 + other.y * w1;
+          m_ref = m;
+        }
+      }
+      __syncwarp();
+      if (!__all_sync(0xffffffffu, ok)) {
+        fail();
+        break;
+      }
+      if (mine) {
+        tc_fence_after();
+        const bool whole = g.j0 == 0 && g.j1 == g.s.nt;
+        const bool odd = *reinterpret_cast<volatile int*>(&s_odd[si & 3]) == si + 1;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // a row that sees nothing: O is 0
+        // A cut item: this part's place (0: the block's run starts in it).
+        const bool from_start = g.j0 != 0 || si == 0;
+        const int64_t slot = (int64_t(blockIdx.x) * 2 + (from_start ? 0 : 1)) * (Wide ? 2 : 1) + (Wide ? t : 0);
+        float4* po = reinterpret_cast<float4*>(a.parts + slot * L::kPart);
+        float2* pm = reinterpret_cast<float2*>(a.parts + slot * L::kPart + size_t(D / 4) * 128 * 16);
+        uint16_t* orow = a.out + (qrow * a.heads + g.kvh * a.group + head) * D;
+        if (warp_live) {
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            float o[32];
+            {
+              uint32_t r[32];
+              tmem_ld32(tO + uint32_t((Wide ? t * D : 0) + c * 32), r);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __uint_as_float(r[e]);
+            }
+            if (!Wide && n > 1) {
+              uint32_t r[32];
+              tmem_ld32(tO + uint32_t(D + c * 32), r);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = o[e] * w0 + __uint_as_float(r[e]) * w1;
+            }
+            if (odd && live) {
+              for (int j = max(0, (g.j0 - g.s.prefix) * kTile); j < min(g.s.count, (g.j1 - g.s.prefix) * kTile); ++j) {
+                if (!(a.mask[qrow * a.words + j / 32] >> (j % 32) & 1)) continue;
+                const uint32_t* v = reinterpret_cast<const uint32_t*>(
+                    a.v_new + ((int64_t(g.b) * a.tokens + j) * a.kv_heads + g.kvh) * D + c * 32);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                  const uint32_t x = split_finite(v[e], true);
+                  o[2 * e] += bf_lo(x);
+                  o[2 * e + 1] += bf_hi(x);
+                }
+              }
+            }
+            if (live && whole) {
+#pragma unroll
+              for (int v = 0; v < 4; ++v) {
+                uint32_t w4[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w4[e] = pack_bf2(o[8 * v + 2 * e] * inv, o[8 * v + 2 * e + 1] * inv);
+                *reinterpret_cast<uint4*>(orow + c * 32 + 8 * v) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
+              }
+            } else if (live) {
+#pragma unroll
+              for (int v = 0; v < 8; ++v)
+                po[(c * 8 + v) * 128 + row] = make_float4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
+            }
+          }
+          if (live && !whole) pm[row] = make_float2(m_ref, l);
+        }
+        // O has been read: the next segment's first P V may overwrite it (the
+        // arrival that lets it start is ordered after this fence).
+        tc_fence_before();
+      }
+      if (!Wide) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(o1_free);
+      }
+      ++si;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
+  if (threadIdx.x == 0 && s_fail && a.err) atomicExch(a.err, 4);
+}
+
+// Joins the parts of the item that block c's run starts in the middle of, when
+// c is the first block whose run does.  Thread = query row, blockIdx.y = 32
+// columns of one query tile.
+template <int D, bool Wide>
+__global__ void __launch_bounds__(128) tree_join_kernel(const Args a) {
+  using L = Lay<D>;
+  pdl_trigger();
+  pdl_wait();
+  const int c = int(blockIdx.x), row = int(threadIdx.x);
+  const int t = Wide ? int(blockIdx.y) / (D / 32) : 0, col = int(blockIdx.y) % (D / 32);
+  const Meta m = a.meta[c];
+  if (m.j0 == 0 || m.j0 > m.chunk) return;
+  const Seq s = seq_of(a, m.b, 1);
+  const int tok = m.pair * a.tpt * (Wide ? 2 : 1) + t * a.tpt + row / a.group;
+  if (row / a.group >= a.tpt || tok >= s.count) return;
+  const int parts = 2 + (m.nt - m.j0 - 1) / m.chunk;  // block c - 1's, then c, c + 1, ...
+  auto place = [&](int k) {
+    const int64_t slot = (int64_t(c - 1 + k) * 2 + (k == 0 && m.j0 < m.chunk ? 1 : 0)) * (Wide ? 2 : 1) + t;
+    return a.parts + slot * L::kPart;
+  };
+  float best = -INFINITY;
+  for (int k = 0; k < parts; ++k)
+    best = fmaxf(best, reinterpret_cast<const float2*>(place(k) + size_t(D / 4) * 128 * 16)[row].x);
+  float l = 0.0f, o[32];
+#pragma unroll
+  for (int e = 0; e < 32; ++e) o[e] = 0.0f;
+  for (int k = 0; k < parts; ++k) {
+    const uint8_t* p = place(k);
+    const float2 ml = reinterpret_cast<const float2*>(p + size_t(D / 4) * 128 * 16)[row];
+    // A part that sees nothing has O = 0, or a non-finite node's value.
+    const float w = best == -INFINITY || ml.x == best ? 1.0f : ex2(ml.x - best);
+    l += w * ml.y;
+    const float4* po = reinterpret_cast<const float4*>(p) + col * 8 * 128 + row;
+#pragma unroll
+    for (int v = 0; v < 8; ++v) {
+      const float4 x = po[v * 128];
+      o[4 * v] += w * x.x;
+      o[4 * v + 1] += w * x.y;
+      o[4 * v + 2] += w * x.z;
+      o[4 * v + 3] += w * x.w;
+    }
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  uint16_t* orow = a.out + ((int64_t(m.b) * a.tokens + tok) * a.heads + m.kvh * a.group + row % a.group) * D + col * 32;
+#pragma unroll
+  for (int v = 0; v < 4; ++v) {
+    uint32_t w4[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w4[e] = pack_bf2(o[8 * v + 2 * e] * inv, o[8 * v + 2 * e + 1] * inv);
+    *reinterpret_cast<uint4*>(orow + 8 * v) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
+  }
+}
+
+constexpr size_t kMetaBytes = size_t(kNumSMs) * sizeof(Meta);
+
+template <int D, bool Wide>
+int launch(const TreeArgs& t, cudaStream_t st) {
+  using L = Lay<D>;
+  static PerDeviceOnce configured;
+  if (!configured.run([] {
+        return cudaFuncSetAttribute(tree_attention_kernel<D, Wide>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    L::kBytes) == cudaSuccess;
+      }))
+    return SB_INTERNAL;
+  const int group = int(t.heads / t.kv_heads), tpt = kTile / group;
+  const bool paged = t.kp.paged();
+  const uint64_t rows = uint64_t(t.batch) * uint64_t(t.tokens);
+  const uint64_t kv_rows = paged ? uint64_t(t.kp.num_pages) * uint64_t(t.kv_heads) * uint64_t(t.kp.page_size)
+                                 : uint64_t(t.batch) * uint64_t(t.kv_heads) * uint64_t(t.max_len);
+  const uint32_t box = paged ? uint32_t(std::min(t.kp.page_size, kTile)) : uint32_t(kTile);
+  auto map = [](CUtensorMap* m, const void* p, uint64_t r, uint64_t cols, uint32_t b) {
+    return make_map_2d(m, p, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, r, cols, 64, b, CU_TENSOR_MAP_SWIZZLE_128B);
+  };
+  CUtensorMap qm, km, vm, knm, vnm;
+  if (!make_map_3d_bf16(&qm, t.q, D, uint64_t(t.heads), rows, uint32_t(group), uint32_t(tpt)) ||
+      !map(&km, t.k_cache, kv_rows, D, box) || !map(&vm, t.v_cache, kv_rows, D, box) ||
+      !map(&knm, t.k_new, rows, uint64_t(t.kv_heads) * D, kTile) ||
+      !map(&vnm, t.v_new, rows, uint64_t(t.kv_heads) * D, kTile))
+    return SB_INTERNAL;
+  Args a{t.base, t.count, t.mask, t.k_new, t.v_new, t.k_cache, t.v_cache, t.out, int(t.batch), int(t.tokens),
+         int(t.heads), int(t.kv_heads), int(t.max_len), group, tpt, int((t.tokens + 31) / 32), t.kp, int(kv_rows),
+         static_cast<Meta*>(t.workspace), static_cast<uint8_t*>(t.workspace) + kMetaBytes, t.err};
+  // A block per SM, fewer when there are not that many tiles even at full lengths.
+  const int per_item = tpt * (Wide ? 2 : 1);
+  const int64_t tiles = (t.max_len + kTile - 1) / kTile + (t.tokens + kTile - 1) / kTile;
+  const int64_t most = t.batch * t.kv_heads * ((t.tokens + per_item - 1) / per_item) * tiles;
+  const unsigned grid = unsigned(std::min<int64_t>(most, kNumSMs));
+  if (launch_pdl(tree_attention_kernel<D, Wide>, dim3(grid), dim3(kThreads), size_t(L::kBytes), st, qm, km, vm, knm,
+                 vnm, a) != cudaSuccess)
+    return SB_INTERNAL;
+  count_launch();
+  if (grid == 1) return SB_OK;  // nothing is cut
+  if (launch_pdl(tree_join_kernel<D, Wide>, dim3(grid, unsigned(D / 32 * (Wide ? 2 : 1))), dim3(128), 0, st, a) !=
+      cudaSuccess)
+    return SB_INTERNAL;
+  count_launch();
+  return SB_OK;
+}
+
+bool wide(int64_t tokens, int64_t heads, int64_t kv_heads) {
+  const int64_t group = heads / kv_heads;
+  return tokens > kTile / group;
 }
 
 }  // namespace
 
-uint64_t tree_attention_workspace_bytes(int64_t, int64_t, int64_t, int64_t) { return 256; }
+uint64_t tree_attention_workspace_bytes(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim) {
+  const uint64_t part = head_dim == 128 ? Lay<128>::kPart : Lay<64>::kPart;
+  return kMetaBytes + uint64_t(kNumSMs) * 2 * part * (wide(tokens, heads, kv_heads) ? 2 : 1);
+}
 
 bool tree_attention_supported(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim) {
   return tokens >= 1 && tokens <= kTreeMaxTokens && kv_heads >= 1 && heads >= 1 && heads % kv_heads == 0 &&
-         heads / kv_heads <= 128 && heads <= 65535 && (head_dim == 64 || head_dim == 128);
+         heads / kv_heads <= kTile && heads <= 65535 && (head_dim == 64 || head_dim == 128);
 }
 
 int launch_tree_attention(const TreeArgs& a, cudaStream_t st) {
   if (!tree_attention_supported(a.tokens, a.heads, a.kv_heads, a.head_dim)) return SB_INVALID_ARGUMENT;
   if (a.batch == 0) return SB_OK;
-  tree_append_kernel<<<dim3(unsigned(a.tokens), unsigned(a.batch)), 128, 0, st>>>(a);
-  SB_LAUNCH_CHECK();
-  tree_warp_kernel<<<dim3(unsigned(a.tokens), unsigned((a.heads + 3) / 4), unsigned(a.batch)), dim3(32, 4), 0, st>>>(a);
-  SB_LAUNCH_CHECK();
-  return SB_OK;
+  if (wide(a.tokens, a.heads, a.kv_heads))
+    return a.head_dim == 128 ? launch<128, true>(a, st) : launch<64, true>(a, st);
+  return a.head_dim == 128 ? launch<128, false>(a, st) : launch<64, false>(a, st);
 }
 
 }  // namespace sb
