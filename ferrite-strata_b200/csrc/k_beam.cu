@@ -7,14 +7,27 @@
 //
 // Within a beam the order of the candidates is the order of its logits, so
 // one pass over the logits is enough: the first kernel reads a run of one
-// row's logits, keeps its maximum, the sum of exponentials against it and the
-// run's `keep` largest logits; the second joins the runs of a row, turns what
-// is left into scores and selects over the beams.  The read of the logits
-// bounds it (HBM) for large calls, latency for small ones.
+// row's logits, sums exponentials and keeps the run's `keep` largest logits; the
+// second joins the runs of a row, turns what is left into scores and selects
+// over the beams.  The read of the logits bounds it (HBM) for large calls,
+// latency for small ones.
+//
+// The first kernel works a warp at a time, 1024 logits a step, with no barrier
+// until the run's end.  A lane sums exponentials against a reference of its own
+// that moves only when a logit exceeds it by 16 (so the sums need no
+// rescaling in practice), and notes the maximum of its 32 logits of each step.
+// At the end the keep-th largest of the 256 lanes' maxima bounds the answer from
+// below, and in random logits little more than `keep` reach it: only the noted
+// groups of 32 whose maximum does are read again, by a whole warp each, and
+// what reaches the bound goes into a list sorted across the warp's lanes
+// (bitonic networks).  Checking every step against a running bound instead took
+// about as many instructions as the sums (56 us, and 105 with each warp going
+// by its own list, for 512 rows of 128001 bf16, keep 32).
 //
 // Scores are compared in 64 bits: two beams' candidates can lie closer than
 // 32 bits resolve at a score of some tens.  A sum of exponentials is kept in
-// 32 bits over the 32 logits a thread holds and in 64 from there on.
+// 32 bits over the 32 logits a lane holds (in pairs, so that many small terms
+// beside a large one are not each rounded against it) and in 64 from there on.
 #include <algorithm>
 
 #include "common.cuh"
@@ -24,26 +37,26 @@ namespace sb {
 
 namespace {
 
-constexpr int kBmThreads = 256;
-constexpr int kBmPer = 32;                        // logits a thread holds
-constexpr int kBmTile = kBmThreads * kBmPer;      // logits per block step
-constexpr int kBmCap = 1024;                      // candidates taken directly against the running threshold
-constexpr int kBmList = kBeamMaxKeep + (kBeamMaxKeep - 1) * kBmPer + 1;  // the most candidates at once
-static_assert(kBmCap + kBeamMaxKeep <= kBmList, "candidate list");
-constexpr int kMgThreads = 1024;
-constexpr int kMgMost = 65536;  // candidates the joining block takes: beams * runs * keep
+constexpr int kWarps = 8;
+constexpr int kThreads = kWarps * 32;
+constexpr int kPer = 32;           // logits a lane holds
+constexpr int kStep = 32 * kPer;   // logits a warp takes at once
+constexpr int kTile = kWarps * kStep;
+constexpr float kLag = 16.0f;      // how far a logit may exceed a lane's reference
+constexpr int kMaxSteps = 24;      // of a run: one noted maximum per lane and step
+constexpr uint32_t kAll = 0xffffffffu;
 
-// Order-preserving map of a float's bits to unsigned.
+// Order-preserving map of a float's bits to unsigned; -0 counts as 0.
 __device__ __forceinline__ uint32_t ord32(float x) {
-  const uint32_t b = __float_as_uint(x);
+  const uint32_t b = __float_as_uint(x + 0.0f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float unord32(uint32_t u) {
   return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
 }
 
-// A candidate of one row: larger key = larger logit, then lower id.  -inf
-// (and NaN, read as -inf) is never a candidate; key 0 stands for none.
+// A candidate of one row: larger key = larger logit, then lower id.  Key 0
+// stands for none.
 __device__ __forceinline__ uint64_t cand_key(float x, uint32_t id) {
   return (uint64_t(ord32(x)) << 32) | uint32_t(~id);
 }
@@ -53,36 +66,126 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float fmax3(float a, float b, float c) {
+  float m;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+  return m;
+}
+__device__ __forceinline__ uint64_t pack_f2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack_f2(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul_f2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 constexpr float kLog2eF = 1.4426950408889634f;
 
 struct RunStat {
-  double sum;
-  float max;
+  double sum;  // of exp(l - ref)
+  float ref;
   int pad;
 };
 
-// 16 bytes of logits from byte address `p`, which need not be aligned: the one
-// or two aligned 16-byte blocks that hold them, shifted together.  A block is
-// read only if it holds a byte below `end`.
-__device__ __forceinline__ uint4 load16(const uint8_t* p, const uint8_t* end) {
-  const uint32_t mis = uint32_t(reinterpret_cast<uintptr_t>(p)) & 15;
-  const uint4* a = reinterpret_cast<const uint4*>(p - mis);
-  const uint4 lo = __ldg(a);
-  if (mis == 0) return lo;
-  uint4 hi = make_uint4(0, 0, 0, 0);
-  if (reinterpret_cast<const uint8_t*>(a + 1) < end) hi = __ldg(a + 1);
-  uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-  if (mis & 8) {
-#pragma unroll
-    for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+// ---------------------------------------------------------------------------
+// Lists sorted across a warp: entry j * 32 + lane, best first
+// ---------------------------------------------------------------------------
+struct Key {
+  uint64_t k;
+  __device__ static Key none() { return Key{0}; }
+  __device__ bool better(const Key& o) const { return k > o.k; }
+  __device__ Key shfl(int lane) const { return Key{__shfl_sync(kAll, k, lane)}; }
+  __device__ Key shfl_xor(int m) const { return Key{__shfl_xor_sync(kAll, k, m)}; }
+};
+
+// A candidate of a batch entry: the score's order-preserving bits, then the
+// lower place among the entry's candidates (beam, run, rank in the run).  Equal
+// scores of one beam are equal logits, which runs and ranks have in the order
+// of their ids, so this is the order of (beam, token).  Score 0 stands for none.
+struct Scored {
+  uint64_t score;
+  uint32_t place;
+  __device__ static Scored none() { return Scored{0, ~0u}; }
+  __device__ bool better(const Scored& o) const { return score > o.score || (score == o.score && place < o.place); }
+  __device__ Scored shfl(int lane) const { return Scored{__shfl_sync(kAll, score, lane), __shfl_sync(kAll, place, lane)}; }
+  __device__ Scored shfl_xor(int m) const {
+    return Scored{__shfl_xor_sync(kAll, score, m), __shfl_xor_sync(kAll, place, m)};
   }
-  if (mis & 4) {
+};
+__device__ __forceinline__ uint64_t ord64(double x) {
+  const uint64_t b = uint64_t(__double_as_longlong(x + 0.0));
+  return b >> 63 ? ~b : b | uint64_t(1) << 63;
+}
+__device__ __forceinline__ double unord64(uint64_t u) {
+  return __longlong_as_double(int64_t(u >> 63 ? u & ~(uint64_t(1) << 63) : ~u));
+}
+
+// Compare-exchange of all entries with those `stride` further on: the better
+// one goes to the lower place where `up` is set, to the higher one otherwise.
+template <typename E, int N>
+__device__ __forceinline__ void exchange(E (&v)[N], int stride, int block) {
+  const int lane = threadIdx.x & 31;
+  if (stride >= 32) {
+    const int d = stride / 32;
 #pragma unroll
-    for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+    for (int j = 0; j < N; ++j) {
+      if (j & d) continue;
+      const bool up = ((j * 32 + lane) & block) == 0;
+      if (v[j + d].better(v[j]) == up) {
+        const E t = v[j];
+        v[j] = v[j + d];
+        v[j + d] = t;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const E o = v[j].shfl_xor(stride);
+      const bool up = ((j * 32 + lane) & block) == 0;
+      const bool low = (lane & stride) == 0;
+      if (o.better(v[j]) == (low == up)) v[j] = o;
+    }
   }
-  const uint32_t sh = (mis & 2) * 8;
-  return make_uint4(__funnelshift_r(w[0], w[1], sh), __funnelshift_r(w[1], w[2], sh), __funnelshift_r(w[2], w[3], sh),
-                    __funnelshift_r(w[3], w[4], sh));
+}
+
+// Sorts N * 32 entries, best first.
+template <typename E, int N>
+__device__ __forceinline__ void sort_list(E (&v)[N]) {
+#pragma unroll
+  for (int block = 2; block <= N * 32; block *= 2)
+#pragma unroll
+    for (int stride = block / 2; stride > 0; stride /= 2) exchange(v, stride, block == N * 32 ? 0 : block);
+}
+
+// v becomes the best N * 32 of two sorted lists, sorted: the better of v[i]
+// and o[last - i] is a bitonic sequence of exactly those.
+template <typename E, int N>
+__device__ __forceinline__ void merge_list(E (&v)[N], const E (&o)[N]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const E x = o[N - 1 - j].shfl(31 - lane);
+    if (x.better(v[j])) v[j] = x;
+  }
+#pragma unroll
+  for (int stride = N * 16; stride > 0; stride /= 2) exchange(v, stride, 0);
+}
+
+// Entry i of a list, to every lane.
+template <typename E, int N>
+__device__ __forceinline__ E entry(const E (&v)[N], int i) {
+  if (N > 1 && i >= 32) return v[N - 1].shfl(i & 31);
+  return v[0].shfl(i & 31);
 }
 
 template <typename T>
@@ -91,7 +194,7 @@ struct BeamArgs {
   const float* scores;
   const int32_t* done;
   int beams, keep, runs;  // runs: blocks per row
-  int vocab, span;        // span: logits per block, a multiple of kBmTile
+  int vocab, span;        // span: logits per block, a multiple of kTile
   int eos;
   float* out_scores;
   int32_t *out_parent, *out_token, *out_done;
@@ -99,284 +202,380 @@ struct BeamArgs {
   uint64_t* cands;  // [rows][runs][keep], best first, 0 past the last
 };
 
-// The rank of every key among n distinct ones, best first; the first `keep` go
-// to out in order.  All threads.
-__device__ __forceinline__ void select_sorted(const uint64_t* in, int n, int keep, uint64_t* out) {
-  for (int i = threadIdx.x; i < n; i += kBmThreads) {
-    const uint64_t k = in[i];
-    int rank = 0;
-    for (int j = 0; j < n; ++j) rank += in[j] > k;
-    if (rank < keep) out[rank] = k;
-  }
+template <typename T>
+__device__ __forceinline__ float logit_at(const uint8_t* row, int i) {
+  if constexpr (sizeof(T) == 2) return bf2f(reinterpret_cast<const uint16_t*>(row)[i]);
+  else return reinterpret_cast<const float*>(row)[i];
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kBmThreads) beam_run_kernel(const BeamArgs<T> a) {
-  constexpr int kVec = 16 / int(sizeof(T));
-  __shared__ uint64_t s_list[kBmList];
-  __shared__ uint64_t s_best[kBeamMaxKeep];
-  __shared__ uint64_t s_tkey[kBmThreads], s_cut;
-  __shared__ double s_red[kBmThreads / 32];
-  __shared__ float s_max[kBmThreads / 32];
-  __shared__ int s_n;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+// 16 bytes at a byte offset `Words` * 4 + (sh ? 2 : 0) into two aligned blocks.
+template <int Words>
+__device__ __forceinline__ uint4 shift16(const uint4& lo, const uint4& hi, uint32_t sh) {
+  const uint32_t w[9] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w, 0};
+  return make_uint4(__funnelshift_r(w[Words], w[Words + 1], sh), __funnelshift_r(w[Words + 1], w[Words + 2], sh),
+                    __funnelshift_r(w[Words + 2], w[Words + 3], sh), __funnelshift_r(w[Words + 3], w[Words + 4], sh));
+}
+
+// N is 1 for lists of 32 (keep <= 32), 2 for lists of 64.
+template <typename T, int N>
+__global__ void __launch_bounds__(kThreads) beam_run_kernel(const BeamArgs<T> a) {
+  constexpr int kVec = 16 / int(sizeof(T)), kLoads = kPer / kVec;
+  __shared__ Key s_new[kWarps][N * 32];  // logits collected by each warp, then its list
+  __shared__ double s_sum[kWarps];
+  __shared__ float s_ref[kWarps];
+  __shared__ float s_note[kMaxSteps][kThreads];  // the maximum of each lane's logits of each step
+  __shared__ float s_max[kWarps][N * 32];
+  __shared__ float s_bound;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int run = blockIdx.x, row = blockIdx.y;
+  const int v0 = run * a.span, v1 = min(a.vocab, v0 + a.span);
   pdl_trigger();
   pdl_wait();
   const float score = a.scores[row];
   if (!(score > -INFINITY) || (a.done && a.done[row])) return;  // no candidate of this row is looked at
-  const int v0 = run * a.span, v1 = min(a.vocab, v0 + a.span);
   const uint8_t* base = reinterpret_cast<const uint8_t*>(a.logits + int64_t(row) * a.vocab);
-  const uint8_t* end = base + int64_t(a.vocab) * int(sizeof(T));
-  float m_run = -INFINITY;
-  double sum = 0.0;   // thread's share, against m_run
-  int have = 0;       // candidates in s_best
-  float tau = -INFINITY;  // the keep-th best so far (have == keep)
-  for (int t0 = v0; t0 < v1; t0 += kBmTile) {
-    float x[kBmPer];
+  // A row may start anywhere.  16 logits' bytes come from the one or two aligned
+  // blocks that hold them, so that lane and place of a logit depend on its id
+  // alone and equal rows give equal sums.
+  const uint32_t mis = uint32_t(reinterpret_cast<uintptr_t>(base)) & 15;
+  const uint4* blocks = reinterpret_cast<const uint4*>(base - mis);
+  const int last_block = int((mis + int64_t(a.vocab) * int(sizeof(T)) - 1) / 16);
+
+  float ref = -INFINITY;
+  double sum = 0.0;
+  float most = -INFINITY;
+  int step = 0;
+  for (int t0 = v0 + warp * kStep; t0 < v1; t0 += kTile) {
+    uint4 u[kLoads];
+    const int blk = t0 / kVec + lane;
+    if (mis == 0) {
 #pragma unroll
-    for (int v = 0; v < kBmPer / kVec; ++v) {
-      const int e = t0 + (v * kBmThreads + tid) * kVec;
-      uint4 u = make_uint4(0, 0, 0, 0);
-      if (e < v1) u = load16(base + int64_t(e) * int(sizeof(T)), end);
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) {
-        float f;
-        if constexpr (sizeof(T) == 2) f = (j & 1) ? bf_hi(w[j / 2]) : bf_lo(w[j / 2]);
-        else f = __uint_as_float(w[j]);
-        x[v * kVec + j] = e + j < v1 ? fmaxf(f, -INFINITY) : -INFINITY;  // NaN -> -inf
-      }
-    }
-    float tm = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < kBmPer; ++i) tm = fmaxf(tm, x[i]);
-    const float wm = warp_max(tm);
-    if (lane == 0) s_max[warp] = wm;
-    if (tid == 0) s_n = 0;
-    __syncthreads();
-    float bm = s_max[0];
-#pragma unroll
-    for (int w = 1; w < kBmThreads / 32; ++w) bm = fmaxf(bm, s_max[w]);
-    // ---- sum of exponentials against the running maximum -----------------------
-    const float m_new = fmaxf(m_run, bm);
-    if (m_new == -INFINITY) {  // nothing but -inf so far
-      __syncthreads();
-      continue;
-    }
-    // In pairs, so that many small terms beside a large one are not each
-    // rounded against it (32 in a row were off by 28 halves of its last bit).
-    float part = 0.0f, quad[kBmPer / 8];
-    if (m_new == INFINITY) {  // only the infinite logits share the probability
-#pragma unroll
-      for (int i = 0; i < kBmPer; ++i) part += x[i] == INFINITY ? 1.0f : 0.0f;
-      sum = m_run == INFINITY ? sum : 0.0;
+      for (int i = 0; i < kLoads; ++i) u[i] = __ldg(blocks + min(blk + i * 32, last_block));
     } else {
+      uint4 hi[kLoads];
 #pragma unroll
-      for (int i = 0; i < kBmPer; i += 8) {
-        float e[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) e[j] = ex2((x[i + j] - m_new) * kLog2eF);
-        quad[i / 8] = ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+      for (int i = 0; i < kLoads; ++i) {
+        u[i] = __ldg(blocks + min(blk + i * 32, last_block));
+        hi[i] = __ldg(blocks + min(blk + i * 32 + 1, last_block));
       }
-      part = (quad[0] + quad[1]) + (quad[2] + quad[3]);
-      if (m_new != m_run) sum = m_run == -INFINITY ? 0.0 : sum * exp(double(m_run) - double(m_new));
-    }
-    sum += double(part);
-    m_run = m_new;
-    // ---- candidates ------------------------------------------------------------
-    // With a full list only logits above its last one count (an equal one has
-    // a higher id).  Without, or when too many are above, the keep-th best of
-    // the threads' best ones is a bound that at least `keep` logits reach; a
-    // thread can hold several logits past it only if its best one is past it,
-    // so at most (keep - 1) * 32 + 1 do.
-    bool direct = have == a.keep;
-    if (direct) {
-      int above = 0;
+      const uint32_t sh = (mis & 2) * 8;
 #pragma unroll
-      for (int i = 0; i < kBmPer; ++i) above += x[i] > tau;
-      if (above) atomicAdd(&s_n, above);
-      __syncthreads();
-      const int n = s_n;
-      if (n == 0) {
-        __syncthreads();
-        continue;
-      }
-      direct = n <= kBmCap;
-    }
-    auto id_of = [&](int i) { return uint32_t(t0 + ((i / kVec) * kBmThreads + tid) * kVec + i % kVec); };
-    uint64_t cut = 0;
-    if (!direct) {
-      int first = 0;
-#pragma unroll
-      for (int i = kBmPer - 1; i >= 0; --i)
-        if (x[i] == tm) first = i;
-      const uint64_t key = tm > -INFINITY ? cand_key(tm, id_of(first)) : 0;
-      s_tkey[tid] = key;
-      if (tid == 0) s_cut = 0;
-      __syncthreads();
-      int rank = 0;
-      for (int j = 0; j < kBmThreads; ++j) rank += s_tkey[j] > key;
-      if (key && rank == a.keep - 1) s_cut = key;
-      __syncthreads();
-      cut = s_cut;
-    }
-    for (int i = tid; i < have; i += kBmThreads) s_list[i] = s_best[i];
-    __syncthreads();
-    if (tid == 0) s_n = have;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kBmPer; ++i) {
-      const float f = x[i];
-      if (f > (have == a.keep ? tau : -INFINITY)) {
-        const uint64_t k = cand_key(f, id_of(i));
-        if (k >= cut) s_list[atomicAdd(&s_n, 1)] = k;
+      for (int i = 0; i < kLoads; ++i) {
+        switch (mis >> 2) {
+          case 0: u[i] = shift16<0>(u[i], hi[i], sh); break;
+          case 1: u[i] = shift16<1>(u[i], hi[i], sh); break;
+          case 2: u[i] = shift16<2>(u[i], hi[i], sh); break;
+          default: u[i] = shift16<3>(u[i], hi[i], sh); break;
+        }
       }
     }
-    __syncthreads();
-    const int n = s_n;
-    select_sorted(s_list, n, a.keep, s_best);
-    have = min(n, a.keep);
-    __syncthreads();
-    if (have == a.keep) tau = unord32(uint32_t(s_best[a.keep - 1] >> 32));
+    auto id_of = [&](int i, int j) { return t0 + (i * 32 + lane) * kVec + j; };  // logit j of load i
+    auto get = [&](int i, int j) {
+      const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+      if constexpr (sizeof(T) == 2) return (j & 1) ? bf_hi(w[j / 2]) : bf_lo(w[j / 2]);
+      else return __uint_as_float(w[j]);
+    };
+    if (t0 + kStep > v1) {  // the row's or run's end: -inf past it
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+#pragma unroll
+        for (int j = 0; j < kVec; ++j)
+          if (id_of(i, j) >= v1) {
+            if constexpr (sizeof(T) == 2) w[j / 2] = (j & 1) ? (w[j / 2] & 0xffffu) | 0xff800000u
+                                                             : (w[j / 2] & 0xffff0000u) | 0xff80u;
+            else w[j] = 0xff800000u;
+          }
+        u[i] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+    float tm = -INFINITY;  // NaN is passed over
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+#pragma unroll
+      for (int j = 0; j < kVec; j += 2) tm = fmax3(tm, get(i, j), get(i, j + 1));
+    if (tm > ref + kLag || ref == -INFINITY) {
+      if (ref != -INFINITY) sum = tm == INFINITY ? 0.0 : sum * exp(double(ref) - double(tm));
+      ref = tm;
+    }
+    // ---- sum of exponentials ---------------------------------------------------
+    {
+      const uint64_t neg = pack_f2(-ref, -ref), scale = pack_f2(kLog2eF, kLog2eF);
+      uint64_t quad[kPer / 8];
+#pragma unroll
+      for (int g = 0; g < kPer / 8; ++g) {
+        uint64_t e[4];
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          const int k = g * 8 + p * 2;
+          float x0, x1;
+          unpack_f2(mul_f2(add_f2(pack_f2(get(k / kVec, k % kVec), get(k / kVec, k % kVec + 1)), neg), scale), x0, x1);
+          e[p] = pack_f2(ex2(x0), ex2(x1));
+        }
+        quad[g] = add_f2(add_f2(e[0], e[1]), add_f2(e[2], e[3]));
+      }
+      float p0, p1;
+      unpack_f2(add_f2(add_f2(quad[0], quad[1]), add_f2(quad[2], quad[3])), p0, p1);
+      float part = p0 + p1;
+      if (part != part) {  // NaN logits, infinite ones, or nothing but -inf so far
+        part = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i)
+#pragma unroll
+          for (int j = 0; j < kVec; ++j) {
+            const float x = get(i, j);
+            if (x == ref && ref != -INFINITY) part += 1.0f;
+            else if (x > -INFINITY && x < ref) part += ref == INFINITY ? 0.0f : ex2((x - ref) * kLog2eF);
+            else if (x > ref && ref != -INFINITY) part += ex2((x - ref) * kLog2eF);
+          }
+      }
+      sum += double(part);
+    }
+    s_note[step++][threadIdx.x] = tm;
+    most = fmaxf(most, tm);
   }
+  // ---- the bound: the keep-th largest of the lanes' maxima -----------------------
+  float tops[N];
+  tops[0] = most;
+  if (N > 1) tops[N - 1] = -INFINITY;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0) s_red[warp] = sum;
+  for (int block = 2; block <= 32; block *= 2)
+#pragma unroll
+    for (int stride = block / 2; stride > 0; stride /= 2) {
+      const float o = __shfl_xor_sync(kAll, tops[0], stride);
+      tops[0] = ((lane & stride) == 0) == ((lane & (block & 31)) == 0) ? fmaxf(tops[0], o) : fminf(tops[0], o);
+    }
+#pragma unroll
+  for (int half = kWarps / 2; half > 0; half /= 2) {
+    if (warp >= half && warp < 2 * half) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) s_max[warp][j * 32 + lane] = tops[j];
+    }
+    __syncthreads();
+    if (warp < half) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) tops[j] = fmaxf(tops[j], s_max[warp + half][N * 32 - 1 - j * 32 - lane]);
+      if (N > 1) {
+        const float x = tops[0], y = tops[N - 1];
+        tops[0] = fmaxf(x, y);
+        tops[N - 1] = fminf(x, y);
+      }
+#pragma unroll
+      for (int stride = 16; stride > 0; stride /= 2)
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          const float o = __shfl_xor_sync(kAll, tops[j], stride);
+          tops[j] = (lane & stride) == 0 ? fmaxf(tops[j], o) : fminf(tops[j], o);
+        }
+    }
+  }
+  if (warp == 0 && lane == (a.keep - 1) % 32) s_bound = tops[N > 1 && a.keep > 32 ? N - 1 : 0];
   __syncthreads();
-  const int64_t slot = int64_t(row) * a.runs + run;
-  if (tid == 0) {
-    double t = 0.0;
-    for (int w = 0; w < kBmThreads / 32; ++w) t += s_red[w];
-    a.stats[slot] = RunStat{t, m_run, 0};
+  const float bound = s_bound;
+  // ---- the warp's list of the logits that reach it ----------------------------------
+  Key list[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) list[j] = Key::none();
+  Key worst = Key::none();  // list entry keep - 1
+  int pending = 0;          // collected logits
+  auto flush = [&]() {
+    __syncwarp();
+    Key fresh[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) fresh[j] = j * 32 + lane < pending ? s_new[warp][j * 32 + lane] : Key::none();
+    sort_list(fresh);
+    merge_list(list, fresh);
+    worst = entry(list, a.keep - 1);
+    pending = 0;
+    __syncwarp();
+  };
+  for (int s = 0; s < step; ++s) {
+    const float note = s_note[s][threadIdx.x];
+    uint32_t hot = __ballot_sync(kAll, note >= bound && note > -INFINITY);
+    while (hot) {
+      const int h = __ffs(hot) - 1;
+      hot &= hot - 1;
+      const int id = v0 + (s * kWarps + warp) * kStep + ((lane / kVec) * 32 + h) * kVec + lane % kVec;
+      const float x = id < v1 ? logit_at<T>(base, id) : -INFINITY;
+      const Key k{cand_key(x, uint32_t(id))};
+      const uint32_t takes = __ballot_sync(kAll, x >= bound && x > -INFINITY && k.better(worst));
+      if (pending + __popc(takes) > N * 32) flush();
+      if (takes >> lane & 1) s_new[warp][pending + __popc(takes & ((1u << lane) - 1))] = k;
+      pending += __popc(takes);
+    }
   }
-  for (int i = tid; i < a.keep; i += kBmThreads) a.cands[slot * a.keep + i] = i < have ? s_best[i] : 0;
+  if (pending) flush();
+  // ---- the block's sum and list ------------------------------------------------
+  const float top = warp_max(ref);
+  double part = ref == top || sum == 0.0 ? sum : top == INFINITY ? 0.0 : sum * exp(double(ref) - double(top));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(kAll, part, o);
+  if (lane == 0) {
+    s_sum[warp] = part;
+    s_ref[warp] = top;
+  }
+#pragma unroll
+  for (int half = kWarps / 2; half > 0; half /= 2) {
+    __syncthreads();
+    if (warp >= half && warp < 2 * half) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) s_new[warp][j * 32 + lane] = list[j];
+    }
+    __syncthreads();
+    if (warp < half) {
+      Key other[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) other[j] = s_new[warp + half][j * 32 + lane];
+      merge_list(list, other);
+    }
+  }
+  if (warp != 0) return;
+  const int64_t slot = int64_t(row) * a.runs + run;
+  if (lane == 0) {
+    float r = s_ref[0];
+    for (int w = 1; w < kWarps; ++w) r = fmaxf(r, s_ref[w]);
+    double t = 0.0;
+    for (int w = 0; w < kWarps; ++w)
+      t += s_ref[w] == r || s_sum[w] == 0.0 ? s_sum[w] : r == INFINITY ? 0.0 : s_sum[w] * exp(double(s_ref[w]) - double(r));
+    a.stats[slot] = RunStat{t, r, 0};
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    if (j * 32 + lane < a.keep) a.cands[slot * a.keep + j * 32 + lane] = list[j].k;
+  }
 }
 
-// A candidate of a batch entry: better = higher score, then lower `flat`
-// (beam << 32 | token).
-struct Scored {
-  double score;
-  uint64_t flat;
-};
-__device__ __forceinline__ bool better(const Scored& a, const Scored& b) {
-  return a.score > b.score || (a.score == b.score && a.flat < b.flat);
-}
-constexpr uint64_t kNoFlat = ~uint64_t(0);
-
-template <typename T>
-__global__ void __launch_bounds__(kMgThreads) beam_join_kernel(const BeamArgs<T> a) {
+// One block per batch entry; a warp takes every 16th list (a run of a beam) and
+// merges it, as scores, into a list of its own; the warps' lists are joined in
+// pairs.
+constexpr int kJoinWarps = 16;
+template <typename T, int N>
+__global__ void __launch_bounds__(kJoinWarps * 32) beam_join_kernel(const BeamArgs<T> a) {
   extern __shared__ __align__(16) uint8_t smem[];
-  double* s_log = reinterpret_cast<double*>(smem);             // [beams] log of the row's sum
-  float* s_m = reinterpret_cast<float*>(s_log + a.beams);      // [beams] the row's maximum
-  Scored* s_top = reinterpret_cast<Scored*>(smem + ((size_t(a.beams) * 12 + 15) & ~size_t(15)));  // [threads] best of each
-  Scored* s_list = s_top + kMgThreads;                         // survivors
-  __shared__ int s_n;
-  __shared__ Scored s_cut;
-  const int tid = threadIdx.x, b = blockIdx.x;
+  double* s_log = reinterpret_cast<double*>(smem);           // [beams] log of the row's sum
+  float* s_ref = reinterpret_cast<float*>(s_log + a.beams);  // [beams]
+  __shared__ Scored s_list[kJoinWarps][N * 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = blockIdx.x;
   pdl_trigger();
   pdl_wait();
-  if (tid == 0) {
-    s_n = 0;
-    s_cut = Scored{-INFINITY, kNoFlat};
-  }
-  for (int w = tid; w < a.beams; w += kMgThreads) {
+  const int lists = a.beams * a.runs;
+  // The keys of list i, if it is one of a live beam.
+  uint64_t keys[N];
+  float score = -INFINITY;
+  bool ended = false;
+  auto fetch = [&](int i) {
+    const int w = i / a.runs;
     const int64_t row = int64_t(b) * a.beams + w;
-    const bool dead = !(a.scores[row] > -INFINITY), done = a.done && a.done[row];
-    float m = -INFINITY;
+    score = a.scores[row];
+    ended = a.done && a.done[row];
+    const uint64_t* p = a.cands + (row * a.runs + i % a.runs) * a.keep;
+#pragma unroll
+    for (int j = 0; j < N; ++j) keys[j] = j * 32 + lane < a.keep ? p[j * 32 + lane] : 0;
+  };
+  if (warp < lists) fetch(warp);
+  for (int w = threadIdx.x; w < a.beams; w += kJoinWarps * 32) {
+    const int64_t row = int64_t(b) * a.beams + w;
+    float r = -INFINITY;
     double sum = 0.0;
-    if (!dead && !done) {
-      for (int r = 0; r < a.runs; ++r) m = fmaxf(m, a.stats[row * a.runs + r].max);
-      for (int r = 0; r < a.runs; ++r) {
-        const RunStat s = a.stats[row * a.runs + r];
-        if (s.max > -INFINITY) sum += s.max == m ? s.sum : m == INFINITY ? 0.0 : s.sum * exp(double(s.max) - double(m));
+    if (a.scores[row] > -INFINITY && !(a.done && a.done[row])) {
+      for (int k = 0; k < a.runs; ++k) r = fmaxf(r, a.stats[row * a.runs + k].ref);
+      for (int k = 0; k < a.runs; ++k) {
+        const RunStat s = a.stats[row * a.runs + k];
+        if (s.sum != 0.0) sum += s.ref == r ? s.sum : r == INFINITY ? 0.0 : s.sum * exp(double(s.ref) - double(r));
       }
     }
-    s_m[w] = m;
+    s_ref[w] = r;
     s_log[w] = log(sum);
   }
   __syncthreads();
-  // Candidate i of the entry: (beam, run, place) with the place fastest.  A
-  // thread takes i = tid, tid + 1024, ...
-  const int per_beam = a.runs * a.keep, total = a.beams * per_beam;
-  auto get = [&](int i) {
-    const int w = i / per_beam, j = i % per_beam;
+  Scored list[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) list[j] = Scored::none();
+  Scored worst = Scored::none();
+  for (int i = warp; i < lists; i += kJoinWarps) {
+    if (i != warp) fetch(i);
+    const int w = i / a.runs;
+    Scored fresh[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int e = j * 32 + lane;
+      double v = -INFINITY;
+      if (ended) {
+        if (e == 0 && i % a.runs == 0) v = double(score);  // an ended beam's one candidate
+      } else if (score > -INFINITY && keys[j]) {
+        const float x = unord32(uint32_t(keys[j] >> 32)), r = s_ref[w];
+        v = double(score) + ((x == r ? 0.0 : double(x) - double(r)) - s_log[w]);
+      }
+      fresh[j] = v > -INFINITY ? Scored{ord64(v), uint32_t(i * a.keep + e)} : Scored::none();
+    }
+    if (!__any_sync(kAll, fresh[0].better(worst))) continue;  // in order: its first entries are its best
+    merge_list(list, fresh);
+    worst = entry(list, a.keep - 1);
+  }
+#pragma unroll
+  for (int half = kJoinWarps / 2; half > 0; half /= 2) {
+    if (warp >= half && warp < 2 * half) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) s_list[warp][j * 32 + lane] = list[j];
+    }
+    __syncthreads();
+    if (warp < half && warp + half < lists) {
+      Scored other[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) other[j] = s_list[warp + half][j * 32 + lane];
+      merge_list(list, other);
+    }
+  }
+  if (warp != 0) return;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int e = j * 32 + lane;
+    if (e >= a.keep) continue;
+    const int64_t o = int64_t(b) * a.keep + e;
+    const Scored c = list[j];
+    if (c.score == 0) {
+      a.out_scores[o] = -INFINITY;
+      a.out_parent[o] = a.out_token[o] = -1;
+      a.out_done[o] = 0;
+      continue;
+    }
+    const int i = int(c.place) / a.keep, w = i / a.runs;
     const int64_t row = int64_t(b) * a.beams + w;
-    Scored c{-INFINITY, kNoFlat};
-    const float s = a.scores[row];
-    if (!(s > -INFINITY)) return c;
-    if (a.done && a.done[row]) {
-      if (j == 0) c = Scored{double(s), uint64_t(w) << 32 | uint32_t(max(a.eos, 0))};
-      return c;
-    }
-    const uint64_t k = a.cands[row * per_beam + j];
-    if (k == 0) return c;
-    const float x = unord32(uint32_t(k >> 32)), m = s_m[w];
-    c.score = double(s) + ((x == m ? 0.0 : double(x) - double(m)) - s_log[w]);
-    c.flat = uint64_t(w) << 32 | uint32_t(~uint32_t(k));
-    if (!(c.score > -INFINITY)) c = Scored{-INFINITY, kNoFlat};
-    return c;
-  };
-  Scored best{-INFINITY, kNoFlat};
-  for (int i = tid; i < total; i += kMgThreads) {
-    const Scored c = get(i);
-    if (better(c, best)) best = c;
-  }
-  s_top[tid] = best;
-  __syncthreads();
-  // The keep-th best of the threads' best ones bounds the answer from below.
-  const int live = min(total, kMgThreads);
-  if (tid < live && best.flat != kNoFlat) {
-    int rank = 0;
-    for (int j = 0; j < live; ++j) rank += better(s_top[j], best);
-    if (rank == a.keep - 1) s_cut = best;
-  }
-  __syncthreads();
-  const Scored cut = s_cut;
-  if (best.flat != kNoFlat && !better(cut, best)) {
-    for (int i = tid; i < total; i += kMgThreads) {
-      const Scored c = get(i);
-      if (c.flat != kNoFlat && !better(cut, c)) s_list[atomicAdd(&s_n, 1)] = c;
-    }
-  }
-  __syncthreads();
-  const int n = s_n;
-  const int64_t o0 = int64_t(b) * a.keep;
-  for (int i = tid; i < n; i += kMgThreads) {
-    const Scored c = s_list[i];
-    int rank = 0;
-    for (int j = 0; j < n; ++j) rank += better(s_list[j], c);
-    if (rank < a.keep) {
-      const int w = int(c.flat >> 32), token = int(uint32_t(c.flat));
-      const int64_t row = int64_t(b) * a.beams + w;
-      const bool done = a.done && a.done[row];
-      a.out_scores[o0 + rank] = float(c.score);
-      a.out_parent[o0 + rank] = int(row);
-      a.out_token[o0 + rank] = done && a.eos < 0 ? -1 : token;
-      a.out_done[o0 + rank] = done || (a.eos >= 0 && token == a.eos) ? 1 : 0;
-    }
-  }
-  for (int i = n + tid; i < a.keep; i += kMgThreads) {
-    a.out_scores[o0 + i] = -INFINITY;
-    a.out_parent[o0 + i] = -1;
-    a.out_token[o0 + i] = -1;
-    a.out_done[o0 + i] = 0;
+    const bool done = a.done && a.done[row];
+    const int token =
+        done ? a.eos : int(~uint32_t(a.cands[(row * a.runs + i % a.runs) * a.keep + int(c.place) % a.keep]));
+    a.out_scores[o] = float(unord64(c.score));
+    a.out_parent[o] = int(row);
+    a.out_token[o] = token;
+    a.out_done[o] = done || token == a.eos ? 1 : 0;
   }
 }
 
-// Blocks per row: enough for four blocks on every SM, each with at least one
-// tile, at most what the joining block takes.
-int beam_runs(int64_t rows, int64_t beams, int64_t vocab, int64_t keep) {
-  const int64_t tiles = (vocab + kBmTile - 1) / kBmTile;
-  int64_t runs = (4 * kNumSMs + rows - 1) / rows;
-  runs = std::min(runs, tiles);
-  runs = std::min(runs, kMgMost / (beams * keep));
-  runs = std::max<int64_t>(runs, 1);
+// Blocks per row: enough for kRunsPerSm blocks on every SM, each with at least
+// one tile and at most kMaxSteps.
+constexpr int kRunsPerSm = 4;
+int beam_runs(int64_t rows, int64_t vocab) {
+  const int64_t tiles = (vocab + kTile - 1) / kTile;
+  int64_t runs = std::min((kRunsPerSm * kNumSMs + rows - 1) / rows, tiles);
+  runs = std::max(runs, (tiles + kMaxSteps - 1) / kMaxSteps);
   const int64_t per = (tiles + runs - 1) / runs;
   return int((tiles + per - 1) / per);
 }
 
 constexpr uint64_t up256(uint64_t x) { return (x + 255) & ~uint64_t(255); }
+
+template <typename T, int N>
+int launch_beam(const BeamArgs<T>& a, int64_t batch, cudaStream_t st) {
+  if (launch_pdl(beam_run_kernel<T, N>, dim3(unsigned(a.runs), unsigned(batch * a.beams)), dim3(kThreads), 0, st, a) !=
+      cudaSuccess)
+    return SB_INTERNAL;
+  count_launch();
+  if (launch_pdl(beam_join_kernel<T, N>, dim3(unsigned(batch)), dim3(kJoinWarps * 32), size_t(a.beams) * 12, st, a) !=
+      cudaSuccess)
+    return SB_INTERNAL;
+  count_launch();
+  return SB_OK;
+}
 
 }  // namespace
 
@@ -387,7 +586,7 @@ bool beam_select_supported(int64_t batch, int64_t beams, int64_t vocab, int64_t 
 
 uint64_t beam_select_workspace_bytes(int64_t batch, int64_t beams, int64_t vocab, int64_t keep) {
   if (!beam_select_supported(batch, beams, vocab, keep) || batch == 0) return 0;
-  const uint64_t slots = uint64_t(batch * beams) * uint64_t(beam_runs(batch * beams, beams, vocab, keep));
+  const uint64_t slots = uint64_t(batch * beams) * uint64_t(beam_runs(batch * beams, vocab));
   return up256(slots * sizeof(RunStat)) + up256(slots * uint64_t(keep) * sizeof(uint64_t));
 }
 
@@ -398,31 +597,15 @@ int launch_beam_select(const T* logits, const float* scores, const int32_t* done
   if (!beam_select_supported(batch, beams, vocab, keep)) return SB_INVALID_ARGUMENT;
   if (batch == 0) return SB_OK;
   const int64_t rows = batch * beams;
-  const int runs = beam_runs(rows, beams, vocab, keep);
-  const int64_t tiles = (vocab + kBmTile - 1) / kBmTile;
+  const int runs = beam_runs(rows, vocab);
+  const int64_t tiles = (vocab + kTile - 1) / kTile;
   BeamArgs<T> a{logits, scores, done, int(beams), int(keep), runs, int(vocab),
-                int((tiles + runs - 1) / runs * kBmTile), int(eos), out_scores, out_parent, out_token, out_done,
+                int((tiles + runs - 1) / runs * kTile), int(eos), out_scores, out_parent, out_token, out_done,
                 nullptr, nullptr};
   a.stats = static_cast<RunStat*>(workspace);
   a.cands = reinterpret_cast<uint64_t*>(static_cast<uint8_t*>(workspace) +
                                         up256(uint64_t(rows) * uint64_t(runs) * sizeof(RunStat)));
-  if (launch_pdl(beam_run_kernel<T>, dim3(unsigned(runs), unsigned(rows)), dim3(kBmThreads), 0, st, a) != cudaSuccess)
-    return SB_INTERNAL;
-  count_launch();
-  // Survivors of the joining block: fewer than keep threads hold more than one.
-  const int64_t each = (beams * runs * keep + kMgThreads - 1) / kMgThreads;
-  const size_t smem = ((size_t(beams) * 12 + 15) & ~size_t(15)) +
-                      sizeof(Scored) * size_t(kMgThreads + keep * each);
-  static PerDeviceOnce configured;
-  if (!configured.run([] {
-        return cudaFuncSetAttribute(beam_join_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024) ==
-               cudaSuccess;
-      }))
-    return SB_INTERNAL;
-  if (launch_pdl(beam_join_kernel<T>, dim3(unsigned(batch)), dim3(kMgThreads), smem, st, a) != cudaSuccess)
-    return SB_INTERNAL;
-  count_launch();
-  return SB_OK;
+  return keep <= 32 ? launch_beam<T, 1>(a, batch, st) : launch_beam<T, 2>(a, batch, st);
 }
 
 template int launch_beam_select<uint16_t>(const uint16_t*, const float*, const int32_t*, int64_t, int64_t, int64_t,
