@@ -18,11 +18,12 @@
 // rescaling in practice), and notes the maximum of its 32 logits of each step.
 // At the end the keep-th largest of the 256 lanes' maxima bounds the answer from
 // below, and in random logits little more than `keep` reach it: only the noted
-// groups of 32 whose maximum does are read again, by a whole warp each, and
-// what reaches the bound goes into a list sorted across the warp's lanes
-// (bitonic networks).  Checking every step against a running bound instead took
-// about as many instructions as the sums (56 us, and 105 with each warp going
-// by its own list, for 512 rows of 128001 bf16, keep 32).
+// groups of 32 whose maximum does are read again, and what reaches the bound is
+// placed by counting.  Checking every step against a running bound instead took
+// about as many instructions as the sums (56 us, and 105 with each warp going by
+// a list of its own, against 37, for 512 rows of 128001 bf16, keep 32); a ring of
+// asynchronous copies to shared memory cost more in resident blocks than it hid
+// (54 us).  Without the last part the pass takes 28 us, 4.7 TB/s.
 //
 // Scores are compared in 64 bits: two beams' candidates can lie closer than
 // 32 bits resolve at a score of some tens.  A sum of exponentials is kept in
@@ -109,17 +110,15 @@ struct Key {
 };
 
 // A candidate of a batch entry: the score's order-preserving bits, then the
-// lower place among the entry's candidates (beam, run, rank in the run).  Equal
-// scores of one beam are equal logits, which runs and ranks have in the order
-// of their ids, so this is the order of (beam, token).  Score 0 stands for none.
+// lower `flat` (beam << 32 | token).  Score 0 stands for none.
 struct Scored {
   uint64_t score;
-  uint32_t place;
-  __device__ static Scored none() { return Scored{0, ~0u}; }
-  __device__ bool better(const Scored& o) const { return score > o.score || (score == o.score && place < o.place); }
-  __device__ Scored shfl(int lane) const { return Scored{__shfl_sync(kAll, score, lane), __shfl_sync(kAll, place, lane)}; }
+  uint64_t flat;
+  __device__ static Scored none() { return Scored{0, ~uint64_t(0)}; }
+  __device__ bool better(const Scored& o) const { return score > o.score || (score == o.score && flat < o.flat); }
+  __device__ Scored shfl(int lane) const { return Scored{__shfl_sync(kAll, score, lane), __shfl_sync(kAll, flat, lane)}; }
   __device__ Scored shfl_xor(int m) const {
-    return Scored{__shfl_xor_sync(kAll, score, m), __shfl_xor_sync(kAll, place, m)};
+    return Scored{__shfl_xor_sync(kAll, score, m), __shfl_xor_sync(kAll, flat, m)};
   }
 };
 __device__ __forceinline__ uint64_t ord64(double x) {
@@ -216,11 +215,20 @@ __device__ __forceinline__ uint4 shift16(const uint4& lo, const uint4& hi, uint3
                     __funnelshift_r(w[Words + 2], w[Words + 3], sh), __funnelshift_r(w[Words + 3], w[Words + 4], sh));
 }
 
+// Asks for n 16-byte blocks from p on to be brought into L2.
+__device__ __forceinline__ void prefetch_l2(const uint4* p, int n) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(n * 16) : "memory");
+}
+
 // N is 1 for lists of 32 (keep <= 32), 2 for lists of 64.
 template <typename T, int N>
 __global__ void __launch_bounds__(kThreads) beam_run_kernel(const BeamArgs<T> a) {
   constexpr int kVec = 16 / int(sizeof(T)), kLoads = kPer / kVec;
-  __shared__ Key s_new[kWarps][N * 32];  // logits collected by each warp, then its list
+  constexpr int kCollect = kWarps * N * 32;
+  __shared__ Key s_all[kCollect];  // logits that reach the bound
+  constexpr int kHot = 256;
+  __shared__ int s_hot[kHot];  // groups of 32 logits with one that reaches the bound
+  __shared__ int s_count, s_hots;
   __shared__ double s_sum[kWarps];
   __shared__ float s_ref[kWarps];
   __shared__ float s_note[kMaxSteps][kThreads];  // the maximum of each lane's logits of each step
@@ -229,6 +237,7 @@ __global__ void __launch_bounds__(kThreads) beam_run_kernel(const BeamArgs<T> a)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int run = blockIdx.x, row = blockIdx.y;
   const int v0 = run * a.span, v1 = min(a.vocab, v0 + a.span);
+  if (threadIdx.x == 0) s_count = s_hots = 0;
   pdl_trigger();
   pdl_wait();
   const float score = a.scores[row];
@@ -248,6 +257,9 @@ __global__ void __launch_bounds__(kThreads) beam_run_kernel(const BeamArgs<T> a)
   for (int t0 = v0 + warp * kStep; t0 < v1; t0 += kTile) {
     uint4 u[kLoads];
     const int blk = t0 / kVec + lane;
+    // The step after next, on its way to L2.
+    const int ahead = (t0 + 2 * kTile) / kVec;
+    if (lane == 0 && t0 + 2 * kTile < v1) prefetch_l2(blocks + ahead, min(kStep / kVec, last_block + 1 - ahead));
     if (mis == 0) {
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) u[i] = __ldg(blocks + min(blk + i * 32, last_block));
@@ -372,39 +384,40 @@ __global__ void __launch_bounds__(kThreads) beam_run_kernel(const BeamArgs<T> a)
   if (warp == 0 && lane == (a.keep - 1) % 32) s_bound = tops[N > 1 && a.keep > 32 ? N - 1 : 0];
   __syncthreads();
   const float bound = s_bound;
-  // ---- the warp's list of the logits that reach it ----------------------------------
-  Key list[N];
-#pragma unroll
-  for (int j = 0; j < N; ++j) list[j] = Key::none();
-  Key worst = Key::none();  // list entry keep - 1
-  int pending = 0;          // collected logits
-  auto flush = [&]() {
-    __syncwarp();
-    Key fresh[N];
-#pragma unroll
-    for (int j = 0; j < N; ++j) fresh[j] = j * 32 + lane < pending ? s_new[warp][j * 32 + lane] : Key::none();
-    sort_list(fresh);
-    merge_list(list, fresh);
-    worst = entry(list, a.keep - 1);
-    pending = 0;
-    __syncwarp();
+  // ---- the logits that reach it ---------------------------------------------------
+  // The hot groups of all warps, up to kHot; then a warp takes every 8th of
+  // them, four at a time, and the block collects up to kCollect logits.
+  auto group_id = [&](int g) {  // this lane's logit of group g = step * kThreads + thread
+    const int s = g / kThreads, t = g % kThreads;
+    return v0 + (s * kWarps + t / 32) * kStep + ((lane / kVec) * 32 + t % 32) * kVec + lane % kVec;
   };
   for (int s = 0; s < step; ++s) {
     const float note = s_note[s][threadIdx.x];
-    uint32_t hot = __ballot_sync(kAll, note >= bound && note > -INFINITY);
-    while (hot) {
-      const int h = __ffs(hot) - 1;
-      hot &= hot - 1;
-      const int id = v0 + (s * kWarps + warp) * kStep + ((lane / kVec) * 32 + h) * kVec + lane % kVec;
-      const float x = id < v1 ? logit_at<T>(base, id) : -INFINITY;
-      const Key k{cand_key(x, uint32_t(id))};
-      const uint32_t takes = __ballot_sync(kAll, x >= bound && x > -INFINITY && k.better(worst));
-      if (pending + __popc(takes) > N * 32) flush();
-      if (takes >> lane & 1) s_new[warp][pending + __popc(takes & ((1u << lane) - 1))] = k;
-      pending += __popc(takes);
+    if (note >= bound && note > -INFINITY) {
+      const int at = atomicAdd(&s_hots, 1);
+      if (at < kHot) s_hot[at] = s * kThreads + int(threadIdx.x);
     }
   }
-  if (pending) flush();
+  __syncthreads();
+  const int hots = s_hots;
+  if (hots <= kHot) {
+    for (int g0 = warp; g0 < hots; g0 += 4 * kWarps) {
+      float x[4];
+      int id[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int g = g0 + q * kWarps;
+        id[q] = g < hots ? group_id(s_hot[g]) : v1;
+        x[q] = id[q] < v1 ? logit_at<T>(base, id[q]) : -INFINITY;
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (x[q] >= bound && x[q] > -INFINITY) {
+          const int at = atomicAdd(&s_count, 1);
+          if (at < kCollect) s_all[at] = Key{cand_key(x[q], uint32_t(id[q]))};
+        }
+    }
+  }
   // ---- the block's sum and list ------------------------------------------------
   const float top = warp_max(ref);
   double part = ref == top || sum == 0.0 ? sum : top == INFINITY ? 0.0 : sum * exp(double(ref) - double(top));
@@ -414,34 +427,85 @@ __global__ void __launch_bounds__(kThreads) beam_run_kernel(const BeamArgs<T> a)
     s_sum[warp] = part;
     s_ref[warp] = top;
   }
+  __syncthreads();
+  const int count = hots <= kHot ? s_count : kCollect + 1;
+  const int64_t place = int64_t(row) * a.runs + run;
+  uint64_t* out = a.cands + place * a.keep;
+  if (warp == 0) {
+    const float own = s_ref[lane % kWarps], r = warp_max(own);
+    double t = lane < kWarps ? s_sum[lane] : 0.0;
+    if (own != r && t != 0.0) t = r == INFINITY ? 0.0 : t * exp(double(own) - double(r));
 #pragma unroll
-  for (int half = kWarps / 2; half > 0; half /= 2) {
-    __syncthreads();
-    if (warp >= half && warp < 2 * half) {
-#pragma unroll
-      for (int j = 0; j < N; ++j) s_new[warp][j * 32 + lane] = list[j];
-    }
-    __syncthreads();
-    if (warp < half) {
-      Key other[N];
-#pragma unroll
-      for (int j = 0; j < N; ++j) other[j] = s_new[warp + half][j * 32 + lane];
-      merge_list(list, other);
-    }
+    for (int o = kWarps / 2; o > 0; o /= 2) t += __shfl_xor_sync(kAll, t, o);
+    if (lane == 0) a.stats[place] = RunStat{t, r, 0};
   }
-  if (warp != 0) return;
-  const int64_t slot = int64_t(row) * a.runs + run;
-  if (lane == 0) {
-    float r = s_ref[0];
-    for (int w = 1; w < kWarps; ++w) r = fmaxf(r, s_ref[w]);
-    double t = 0.0;
-    for (int w = 0; w < kWarps; ++w)
-      t += s_ref[w] == r || s_sum[w] == 0.0 ? s_sum[w] : r == INFINITY ? 0.0 : s_sum[w] * exp(double(s_ref[w]) - double(r));
-    a.stats[slot] = RunStat{t, r, 0};
-  }
+  if (count <= kCollect) {
+    // A logit's place is the number of better ones.
+    for (int i = int(threadIdx.x); i < max(count, a.keep); i += kThreads) {
+      if (i < count) {
+        const Key k = s_all[i];
+        int rank = 0;
+        for (int j = 0; j < count; ++j) rank += s_all[j].better(k);
+        if (rank < a.keep) out[rank] = k.k;
+      } else {
+        out[i] = 0;
+      }
+    }
+  } else {
+    // Very many equal logits, or a bound far too low: each warp keeps a sorted
+    // list of its own, and the lists are joined in pairs.
+    Key list[N];
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
-    if (j * 32 + lane < a.keep) a.cands[slot * a.keep + j * 32 + lane] = list[j].k;
+    for (int j = 0; j < N; ++j) list[j] = Key::none();
+    Key worst = Key::none();  // list entry keep - 1
+    int pending = 0;          // collected logits
+    Key* mine = s_all + warp * N * 32;
+    auto flush = [&]() {
+      __syncwarp();
+      Key fresh[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) fresh[j] = j * 32 + lane < pending ? mine[j * 32 + lane] : Key::none();
+      sort_list(fresh);
+      merge_list(list, fresh);
+      worst = entry(list, a.keep - 1);
+      pending = 0;
+      __syncwarp();
+    };
+    for (int s = 0; s < step; ++s) {
+      const float note = s_note[s][threadIdx.x];
+      uint32_t hot = __ballot_sync(kAll, note >= bound && note > -INFINITY);
+      while (hot) {
+        const int h = __ffs(hot) - 1;
+        hot &= hot - 1;
+        const int id = group_id(s * kThreads + warp * 32 + h);
+        const float x = id < v1 ? logit_at<T>(base, id) : -INFINITY;
+        const Key k{cand_key(x, uint32_t(id))};
+        const uint32_t takes = __ballot_sync(kAll, x >= bound && x > -INFINITY && k.better(worst));
+        if (pending + __popc(takes) > N * 32) flush();
+        if (takes >> lane & 1) mine[pending + __popc(takes & ((1u << lane) - 1))] = k;
+        pending += __popc(takes);
+      }
+    }
+    if (pending) flush();
+#pragma unroll
+    for (int half = kWarps / 2; half > 0; half /= 2) {
+      __syncthreads();
+      if (warp >= half && warp < 2 * half) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) mine[j * 32 + lane] = list[j];
+      }
+      __syncthreads();
+      if (warp < half) {
+        Key other[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) other[j] = s_all[(warp + half) * N * 32 + j * 32 + lane];
+        merge_list(list, other);
+      }
+    }
+    if (warp != 0) return;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (j * 32 + lane < a.keep) out[j * 32 + lane] = list[j].k;
   }
 }
 
@@ -454,6 +518,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) beam_join_kernel(const BeamAr
   extern __shared__ __align__(16) uint8_t smem[];
   double* s_log = reinterpret_cast<double*>(smem);           // [beams] log of the row's sum
   float* s_ref = reinterpret_cast<float*>(s_log + a.beams);  // [beams]
+  int* s_done = reinterpret_cast<int*>(s_ref + a.beams);     // [beams]
   __shared__ Scored s_list[kJoinWarps][N * 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = blockIdx.x;
   pdl_trigger();
@@ -475,17 +540,23 @@ __global__ void __launch_bounds__(kJoinWarps * 32) beam_join_kernel(const BeamAr
   if (warp < lists) fetch(warp);
   for (int w = threadIdx.x; w < a.beams; w += kJoinWarps * 32) {
     const int64_t row = int64_t(b) * a.beams + w;
-    float r = -INFINITY;
+    // All loads at once; a row that is not looked at leaves its statistics unwritten.
+    const float sc = a.scores[row];
+    const int dn = a.done ? a.done[row] : 0;
+    const RunStat* st = a.stats + row * a.runs;
+    RunStat s0 = st[0];
+    float r = s0.ref;
+    for (int k = 1; k < a.runs; ++k) r = fmaxf(r, st[k].ref);
     double sum = 0.0;
-    if (a.scores[row] > -INFINITY && !(a.done && a.done[row])) {
-      for (int k = 0; k < a.runs; ++k) r = fmaxf(r, a.stats[row * a.runs + k].ref);
+    if (sc > -INFINITY && !dn) {
       for (int k = 0; k < a.runs; ++k) {
-        const RunStat s = a.stats[row * a.runs + k];
+        const RunStat s = k ? st[k] : s0;
         if (s.sum != 0.0) sum += s.ref == r ? s.sum : r == INFINITY ? 0.0 : s.sum * exp(double(s.ref) - double(r));
       }
     }
     s_ref[w] = r;
     s_log[w] = log(sum);
+    s_done[w] = dn != 0;
   }
   __syncthreads();
   Scored list[N];
@@ -500,20 +571,35 @@ __global__ void __launch_bounds__(kJoinWarps * 32) beam_join_kernel(const BeamAr
     for (int j = 0; j < N; ++j) {
       const int e = j * 32 + lane;
       double v = -INFINITY;
+      uint32_t token = ~uint32_t(keys[j]);
       if (ended) {
         if (e == 0 && i % a.runs == 0) v = double(score);  // an ended beam's one candidate
+        token = uint32_t(max(a.eos, 0));
       } else if (score > -INFINITY && keys[j]) {
         const float x = unord32(uint32_t(keys[j] >> 32)), r = s_ref[w];
         v = double(score) + ((x == r ? 0.0 : double(x) - double(r)) - s_log[w]);
       }
-      fresh[j] = v > -INFINITY ? Scored{ord64(v), uint32_t(i * a.keep + e)} : Scored::none();
+      fresh[j] = v > -INFINITY ? Scored{ord64(v), uint64_t(w) << 32 | token} : Scored::none();
     }
-    if (!__any_sync(kAll, fresh[0].better(worst))) continue;  // in order: its first entries are its best
+    // In the order of its logits, so of its scores, unless scores that differ by
+    // less than f64 resolves have become equal.
+    bool off = false;
+    Scored last = Scored::none();
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      Scored left = fresh[j].shfl((lane + 31) & 31);
+      if (j > 0 && lane == 0) left = last;
+      last = fresh[j].shfl(31);
+      off |= (lane || j) && fresh[j].better(left);
+    }
+    if (__any_sync(kAll, off)) sort_list(fresh);
+    if (!__any_sync(kAll, fresh[0].better(worst))) continue;  // its first entries are its best
     merge_list(list, fresh);
     worst = entry(list, a.keep - 1);
   }
 #pragma unroll
   for (int half = kJoinWarps / 2; half > 0; half /= 2) {
+    if (half >= lists) continue;
     if (warp >= half && warp < 2 * half) {
 #pragma unroll
       for (int j = 0; j < N; ++j) s_list[warp][j * 32 + lane] = list[j];
@@ -539,13 +625,11 @@ __global__ void __launch_bounds__(kJoinWarps * 32) beam_join_kernel(const BeamAr
       a.out_done[o] = 0;
       continue;
     }
-    const int i = int(c.place) / a.keep, w = i / a.runs;
-    const int64_t row = int64_t(b) * a.beams + w;
-    const bool done = a.done && a.done[row];
-    const int token =
-        done ? a.eos : int(~uint32_t(a.cands[(row * a.runs + i % a.runs) * a.keep + int(c.place) % a.keep]));
+    const int w = int(c.flat >> 32);
+    const bool done = s_done[w];
+    const int token = done ? a.eos : int(uint32_t(c.flat));
     a.out_scores[o] = float(unord64(c.score));
-    a.out_parent[o] = int(row);
+    a.out_parent[o] = b * a.beams + w;
     a.out_token[o] = token;
     a.out_done[o] = done || token == a.eos ? 1 : 0;
   }
@@ -553,7 +637,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) beam_join_kernel(const BeamAr
 
 // Blocks per row: enough for kRunsPerSm blocks on every SM, each with at least
 // one tile and at most kMaxSteps.
-constexpr int kRunsPerSm = 4;
+constexpr int kRunsPerSm = 3;
 int beam_runs(int64_t rows, int64_t vocab) {
   const int64_t tiles = (vocab + kTile - 1) / kTile;
   int64_t runs = std::min((kRunsPerSm * kNumSMs + rows - 1) / rows, tiles);
@@ -570,7 +654,7 @@ int launch_beam(const BeamArgs<T>& a, int64_t batch, cudaStream_t st) {
       cudaSuccess)
     return SB_INTERNAL;
   count_launch();
-  if (launch_pdl(beam_join_kernel<T, N>, dim3(unsigned(batch)), dim3(kJoinWarps * 32), size_t(a.beams) * 12, st, a) !=
+  if (launch_pdl(beam_join_kernel<T, N>, dim3(unsigned(batch)), dim3(kJoinWarps * 32), size_t(a.beams) * 16, st, a) !=
       cudaSuccess)
     return SB_INTERNAL;
   count_launch();
