@@ -20,19 +20,23 @@
 // depend on timing.  What bounds it: reading the cache (HBM) up to about 128
 // rows a kv head, the softmax between the two products beyond.
 //
-// Block.  Warp 0 loads by TMA through one ring of 128-row tiles in the order
-// they are used (K0, K1, V0, K2, V1, ...); warp 1 issues the products
+// Block.  Warp 0 walks the block's run and loads by TMA through one ring of
+// 128-row tiles in the order they are used (K0, K1, V0, K2, V1, ...); warp 1
+// issues the products
 //   S = Q K^T    (A, B in shared memory; 128 x 128 f32 in TMEM)
 //   O += P V     (A = P in TMEM, written over S; B = the V tile as loaded)
-// and warps 2-5 and 6-9 are two softmax groups, one thread per query row.  With
-// more than 128 rows the two groups take a query tile each and share every KV
-// tile; with up to 128 rows both work for the same query tile, one on the even
-// and one on the odd KV tiles (each with a maximum, sum and O of its own, joined
-// at the end), so that one group's softmax runs during the other's products.
+// warps 2 and 3 append the new rows, and warps 4-11 and 12-19 are two softmax
+// groups: two threads per query row, 64 positions each.  With more than 128 rows
+// the two groups take a query tile each and share every KV tile; with up to 128
+// rows both work for the same query tile, one on the even and one on the odd KV
+// tiles (each with a maximum, sum and O of its own, joined at the end), so that
+// one group's softmax runs during the other's products.
 //
-// Softmax in base 2: O is rescaled in TMEM only when a row's maximum grows by
-// more than 8, so probabilities stay below 2^8; P is rounded to bf16 for the
-// second product, maximum, sum and O are f32.
+// Softmax in base 2: a row's reference moves, and O is rescaled in TMEM, only
+// when a score exceeds the reference by more than 8, so probabilities stay
+// below 2^8.  The two threads of a row agree by one barrier vote per tile that
+// nothing moves; only when something does they exchange their maxima.  P is
+// rounded to bf16 for the second product; reference, sum and O are f32.
 //
 // Masked places.  A masked score becomes -inf whatever it was.  0 * NaN must
 // not reach O either: V rows at or past a tile's end are zeroed in shared
@@ -53,37 +57,55 @@ namespace {
 
 using namespace tc;
 
-constexpr int kTile = 128;  // query rows per tile, positions per KV tile
-constexpr int kThreads = 320;
+constexpr int kTile = 128;   // query rows per tile, positions per KV tile
+constexpr int kHalf = 64;    // positions per softmax thread
+constexpr int kThreads = 640;
+constexpr int kSegs = 4;     // segments the walking warp is ahead at most, rounded up
 constexpr uint32_t kTmemCols = 512;  // S_0, S_1 (128 columns each), O_0, O_1 (head_dim each)
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescale = 8.0f;  // log2 of the largest P before O is rescaled
 
-// Shared memory: two query tiles (both of an item, or one of this segment and
-// one of the next), the ring, the second group's statistics, the barriers.
-template <int D>
+struct Seq {
+  int base, count;  // count 0 where the sequence is unusable or has no nodes
+  int prefix;       // tiles of cached positions
+  int nt;           // all tiles
+  int pairs;        // items per kv head
+};
+
+// A block's stretch of one item: tiles [j0, j1) of nt.
+struct Seg {
+  Seq s;
+  int b, kvh, pair, j0, j1;
+  int last;  // the block's last one
+};
+
+// Shared memory: the item's query tile (two when wide), the ring, the softmax
+// threads' statistics, the next segments, the barriers.
+template <int D, bool Wide>
 struct Lay {
-  static constexpr int kKB = D / 64;             // 64-wide blocks of head_dim
+  static constexpr int kKB = D / 64;              // 64-wide blocks of head_dim
   static constexpr int kBytesTile = 128 * D * 2;  // kKB blocks of [128 rows][128 bytes]
   static constexpr int kSlots = D == 128 ? 5 : 8;
   static constexpr int kQ = 0;
-  static constexpr int kRing = 2 * kBytesTile;
-  static constexpr int kStat = kRing + kSlots * kBytesTile;  // float2 [128]
-  static constexpr int kBar = kStat + 1024;
-  static constexpr int kBars = 2 * kSlots + 14;
-  static constexpr int kBytes = kBar + kBars * 8 + 16 + 1024;
+  static constexpr int kRing = (Wide ? 2 : 1) * kBytesTile;
+  static constexpr int kStat = kRing + kSlots * kBytesTile;  // sum [2 groups][2 halves][128], reference [2][128] (not wide)
+  static constexpr int kSeg = kStat + 4 * 128 * 4 + (Wide ? 0 : 2 * 128 * 4);
+  static constexpr int kBar = kSeg + kSegs * int(sizeof(Seg));
+  static constexpr int kBars = 2 * kSlots + 12 + kSegs;
+  static constexpr int kUse = kBar + kBars * 8 + 8 + 20;  // and the TMEM address, the failure word, four notes
+  static constexpr int kBytes = kUse + 1024 < 232448 ? kUse + 1024 : 232448;
   static constexpr uint32_t kOCol = 256;
-  static_assert(kBytes <= 232448, "shared memory");
-  // One part of a cut item and query tile: O as [D / 4][128 rows] float4, then (max, sum) [128 rows].
+  static_assert(kUse <= 232448 && kBar % 8 == 0, "shared memory");
+  // One part of a cut item and query tile: O as [D / 4][128 rows] float4, then (reference, sum) [128 rows].
   static constexpr size_t kPart = size_t(D / 4) * 128 * 16 + 128 * 8;
 };
 
 // What the joining kernel needs to know of the item a block's run starts in.
 struct Meta {
-  int b, kvh, pair;
+  int b, kvh, pair, count;
   int j0;  // the item's tile the run starts at (0: the run starts with the item)
   int nt;  // tiles of the item
-  int chunk, pad[2];
+  int chunk, pad;
 };
 
 struct Args {
@@ -101,17 +123,8 @@ struct Args {
   int* err;
 };
 
-struct Seq {
-  int base, count;  // count 0 where the sequence is unusable or has no nodes
-  int prefix;       // tiles of cached positions
-  int nt;           // all tiles
-  int pairs;        // items per kv head
-};
-
-__device__ __forceinline__ Seq seq_of(const Args& a, int b, int per_item, bool* bad = nullptr) {
-  Seq s;
-  s.base = a.base[b];
-  s.count = a.count ? a.count[b] : a.tokens;
+__device__ __forceinline__ Seq make_seq(const Args& a, int base, int count, int per_item, bool* bad = nullptr) {
+  Seq s{base, count, 0, 0, 0};
   const bool wrong = s.count < 0 || s.count > a.tokens || s.base < 0 || s.base > a.max_len - s.count;
   if (bad) *bad = wrong;
   if (wrong) s.base = s.count = 0;
@@ -121,36 +134,38 @@ __device__ __forceinline__ Seq seq_of(const Args& a, int b, int per_item, bool* 
   return s;
 }
 
-// A block's stretch of one item: tiles [j0, j1) of nt.
-struct Seg {
-  Seq s;
-  int b, kvh, pair, j0, j1;
-};
+__device__ __forceinline__ Seq seq_of(const Args& a, int b, int per_item, bool* bad = nullptr) {
+  return make_seq(a, a.base[b], a.count ? a.count[b] : a.tokens, per_item, bad);
+}
 
-// Walks the segments of a block's run.
+// Where a block stands in its run.
 struct Walk {
+  Seq s;  // of sequence b
   int b, left;
-  int64_t off;  // within sequence b's tiles
+  uint32_t off;  // within sequence b's tiles
 };
 
+// The next segment; false at the run's end.  The host bounds all tiles of a
+// call below 2^31.
 __device__ __forceinline__ bool next_seg(const Args& a, int per_item, Walk& w, Seg& g) {
   if (w.left <= 0) return false;
   for (;;) {
-    if (w.b >= a.batch) return false;
-    g.s = seq_of(a, w.b, per_item);
-    const int64_t units = int64_t(g.s.nt) * a.kv_heads * g.s.pairs;
+    const uint32_t units = uint32_t(w.s.nt) * uint32_t(a.kv_heads) * uint32_t(w.s.pairs);
     if (w.off < units) break;
-    w.off -= units;  // zero: runs end where sequences do
-    ++w.b;
+    w.off = 0;  // runs end where sequences do
+    if (++w.b >= a.batch) return false;
+    w.s = seq_of(a, w.b, per_item);
   }
+  g.s = w.s;
   g.b = w.b;
-  const int item = int(w.off / g.s.nt);
-  g.j0 = int(w.off % g.s.nt);
-  g.kvh = item / g.s.pairs;
-  g.pair = item % g.s.pairs;
-  g.j1 = min(g.s.nt, g.j0 + w.left);
+  const uint32_t item = w.off / uint32_t(w.s.nt);
+  g.j0 = int(w.off - item * uint32_t(w.s.nt));
+  g.kvh = int(item / uint32_t(w.s.pairs));
+  g.pair = int(item - uint32_t(g.kvh) * uint32_t(w.s.pairs));
+  g.j1 = min(w.s.nt, g.j0 + w.left);
   w.left -= g.j1 - g.j0;
-  w.off += g.j1 - g.j0;
+  w.off += uint32_t(g.j1 - g.j0);
+  g.last = w.left <= 0;
   return true;
 }
 
@@ -202,9 +217,10 @@ __device__ __forceinline__ uint32_t split_finite(uint32_t v, bool keep) {
 }
 
 // Appends the block's share of the new rows, and zeroes the output rows of
-// dead nodes.  Threads 0..255 (the softmax groups').
+// dead nodes.  Threads 0..63.
 template <int D>
 __device__ void append_rows(const Args& a, int tid) {
+  constexpr int kT = 64, kU = 4;  // threads; pieces in flight of each
   constexpr int kPer = D / 8;  // 16-byte pieces per head
   const int rows = a.batch * a.tokens, pieces = a.kv_heads * kPer;
   for (int r = int(blockIdx.x); r < rows; r += int(gridDim.x)) {
@@ -214,22 +230,52 @@ __device__ void append_rows(const Args& a, int tid) {
     if (bad && t == 0 && tid == 0 && a.err) atomicExch(a.err, kBadPosition);
     if (t >= s.count) {
       uint4* o = reinterpret_cast<uint4*>(a.out) + int64_t(r) * a.heads * kPer;
-      for (int i = tid; i < a.heads * kPer; i += 256) o[i] = make_uint4(0, 0, 0, 0);
+      for (int i = tid; i < a.heads * kPer; i += kT) o[i] = make_uint4(0, 0, 0, 0);
       continue;
     }
     const uint4* kn = reinterpret_cast<const uint4*>(a.k_new) + int64_t(r) * pieces;
     const uint4* vn = reinterpret_cast<const uint4*>(a.v_new) + int64_t(r) * pieces;
-    for (int i = tid; i < pieces; i += 256) {
-      const int64_t row = kv_row(a.kp, b, i / kPer, a.kv_heads, a.max_len, s.base + t);
-      if (row < 0) {
-        if (a.err) atomicExch(a.err, kBadPage);
-        continue;
-      }
-      const uint4 k = kn[i], v = vn[i];
-      reinterpret_cast<uint4*>(a.k_cache)[row * kPer + i % kPer] = k;
-      reinterpret_cast<uint4*>(a.v_cache)[row * kPer + i % kPer] = v;
+    const int64_t row0 = kv_row(a.kp, b, 0, a.kv_heads, a.max_len, s.base + t);
+    if (row0 < 0) {
+      if (tid == 0 && a.err) atomicExch(a.err, kBadPage);
+      continue;
+    }
+    const int64_t step = a.kp.paged() ? a.kp.page_size : a.max_len;  // rows between kv heads
+    for (int i0 = tid; i0 < pieces; i0 += kT * kU) {
+      uint4 k[kU], v[kU];
+#pragma unroll
+      for (int u = 0; u < kU; ++u)
+        if (i0 + u * kT < pieces) {
+          k[u] = kn[i0 + u * kT];
+          v[u] = vn[i0 + u * kT];
+        }
+#pragma unroll
+      for (int u = 0; u < kU; ++u)
+        if (i0 + u * kT < pieces) {
+          const int i = i0 + u * kT;
+          const int64_t at = (row0 + i / kPer * step) * kPer + i % kPer;
+          reinterpret_cast<uint4*>(a.k_cache)[at] = k[u];
+          reinterpret_cast<uint4*>(a.v_cache)[at] = v[u];
+        }
     }
   }
+}
+
+// Whether `p` holds in any thread of the two warps that share barrier `id`.
+__device__ __forceinline__ bool pair_any(int id, bool p) {
+  uint32_t r;
+  __syncwarp();
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n bar.red.or.pred q, %2, 64, p;\n selp.u32 %0, 1, 0, q;\n}"
+      : "=r"(r)
+      : "r"(uint32_t(p)), "r"(id)
+      : "memory");
+  return r != 0;
+}
+
+__device__ __forceinline__ void pair_sync(int id) {
+  __syncwarp();
+  asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory");
 }
 
 template <int D, bool Wide>
@@ -237,26 +283,33 @@ __global__ void __launch_bounds__(kThreads, 1)
     tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                           const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap knmap,
                           const __grid_constant__ CUtensorMap vnmap, const Args a) {
-  using L = Lay<D>;
+  using L = Lay<D, Wide>;
   constexpr int kNS = L::kSlots;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (su32(smem_raw) & 1023u)) & 1023u);
+  if (smem - smem_raw + L::kUse > L::kBytes) {  // the 128-byte swizzle needs the tiles on 1024 bytes
+    if (threadIdx.x == 0 && a.err) atomicExch(a.err, 4);
+    return;
+  }
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBar);
-  uint64_t* full = bars;                // [kNS] ring slot loaded
-  uint64_t* empty = bars + kNS;         // [kNS] ring slot read by its products
-  uint64_t* q_full = bars + 2 * kNS;    // [2]
-  uint64_t* q_empty = q_full + 2;       // [2]
-  uint64_t* s_full = q_full + 4;        // [2] per group: S is in TMEM
-  uint64_t* p_full = q_full + 6;        // [2] per group: P is in TMEM (4 warps arrive)
-  uint64_t* o_done = q_full + 8;        // [2] per group: the segment's last P V is complete
-  uint64_t* st_full = q_full + 10;      // the second group's statistics are written (4 warps)
-  uint64_t* o1_free = q_full + 11;      // the first group has read O_1 and the statistics (4 warps)
-  uint64_t* mma_done = q_full + 12;     // every product of the block is complete
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + L::kBars);
-  float2* stat = reinterpret_cast<float2*>(smem + L::kStat);
-  __shared__ int s_fail;
-  __shared__ int s_odd[4];  // s_odd[i % 4] == i + 1: segment i holds non-finite node values
-  __shared__ Walk s_walk;
+  uint64_t* full = bars;              // [kNS] ring slot loaded
+  uint64_t* empty = bars + kNS;       // [kNS] ring slot read by its products
+  uint64_t* seg_full = bars + 2 * kNS;  // [kSegs] segment written
+  uint64_t* q_full = seg_full + kSegs;  // the segment's query tiles are loaded
+  uint64_t* q_empty = q_full + 1;     // its S products are complete
+  uint64_t* s_full = q_full + 2;      // [2] per group: S is in TMEM
+  uint64_t* p_full = q_full + 4;      // [2] per group: P is in TMEM (8 warps arrive)
+  uint64_t* o_done = q_full + 6;      // [2] per group: the segment's last P V is complete
+  uint64_t* st_full = q_full + 8;     // [2] per group: its statistics are written (8 warps)
+  uint64_t* o_free = q_full + 10;     // O and the statistics have been read (16 warps)
+  uint64_t* mma_done = q_full + 11;   // every product of the block is complete
+  int* words = reinterpret_cast<int*>(bars + L::kBars);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(words);
+  int* s_fail = words + 1;
+  int* s_odd = words + 2;  // [4]: s_odd[i % 4] == i + 1: segment i holds non-finite node values
+  float* s_sum = reinterpret_cast<float*>(smem + L::kStat);  // [group][half][row]
+  float* s_ref = s_sum + 4 * 128;                            // [group][row], not wide
+  Seg* s_seg = reinterpret_cast<Seg*>(smem + L::kSeg);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int per_item = a.tpt * (Wide ? 2 : 1);
@@ -266,17 +319,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
+    for (int s = 0; s < kSegs; ++s) mbar_init(&seg_full[s], 1);
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&q_full[s], 1);
-      mbar_init(&q_empty[s], 1);
       mbar_init(&s_full[s], 1);
-      mbar_init(&p_full[s], 4);
+      mbar_init(&p_full[s], 8);
       mbar_init(&o_done[s], 1);
+      mbar_init(&st_full[s], 8);
     }
-    mbar_init(st_full, 4);
-    mbar_init(o1_free, 4);
+    mbar_init(o_free, 16);
     mbar_init(mma_done, 1);
-    s_fail = 0;
+    *s_fail = 0;
     s_odd[0] = s_odd[1] = s_odd[2] = s_odd[3] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     prefetch_map(&qmap);
@@ -292,35 +346,53 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   pdl_trigger();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
   pdl_wait();  // every operand may come from the kernels before
+  auto fail = [&]() { atomicExch(s_fail, 1); };
+  auto failed = [&]() { return *reinterpret_cast<volatile int*>(s_fail) != 0; };
+
+  // Every role takes the same segments from warp 0 and counts ring loads, S
+  // tiles and segments for itself, so each barrier's phase is known without
+  // any block-wide synchronisation.  Ring loads of a segment of n tiles that
+  // starts at load c0:  K_0: c0;  K_j: c0 + 2j - 1;  V_j: c0 + 2j + 2, the last
+  // one c0 + 2n - 1.  A segment's slot is written again four segments later:
+  // then warp 0 has waited for the S products of two segments later, before
+  // which warp 1 has waited for every softmax warp to be done with this one.
+  auto wait_seg = [&](int si) { return mbar_wait(&seg_full[si % kSegs], (si / kSegs) & 1); };
   if (warp == 0) {
-    // All tiles in one line; this block's run starts in sequence b at tile off.
-    int64_t total = 0;
-    for (int b0 = 0; b0 < a.batch; b0 += 32) {
-      int64_t u = 0;
-      if (b0 + lane < a.batch) {
-        const Seq s = seq_of(a, b0 + lane, per_item);
-        u = int64_t(s.nt) * a.kv_heads * s.pairs;
+    // ---- the walk and the loads --------------------------------------------------
+    // All tiles in one line, an equal run of it per block.
+    const int step = 32;
+    uint32_t total = 0;
+    int base = 0, count = 0;
+    auto units_of = [&](int b) {
+      base = count = 0;
+      if (b < a.batch) {
+        base = a.base[b];
+        count = a.count ? a.count[b] : a.tokens;
       }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
-      total += u;
+      const Seq s = make_seq(a, base, count, per_item);
+      return uint32_t(s.nt) * uint32_t(a.kv_heads) * uint32_t(s.pairs);
+    };
+    uint32_t u = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += step) {
+      u = units_of(b0 + lane);
+      total += __reduce_add_sync(0xffffffffu, u);
     }
-    const int64_t chunk = (total + gridDim.x - 1) / gridDim.x;
-    const int64_t w0 = chunk * blockIdx.x;
-    Walk w{a.batch, 0, 0};
+    const uint32_t chunk = (total + gridDim.x - 1) / gridDim.x;
+    const uint32_t w0 = chunk * blockIdx.x;
+    Walk w{Seq{}, a.batch, 0, 0};
     if (w0 < total) {
-      int64_t before = 0;
-      for (int b0 = 0; b0 < a.batch; b0 += 32) {
-        int64_t u = 0;
-        if (b0 + lane < a.batch) {
-          const Seq s = seq_of(a, b0 + lane, per_item);
-          u = int64_t(s.nt) * a.kv_heads * s.pairs;
-        }
-        int64_t end = u;
+      uint32_t before = 0;
+      for (int b0 = 0; b0 < a.batch; b0 += step) {
+        if (a.batch > step) u = units_of(b0 + lane);
+        uint32_t end = u;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-          const int64_t y = __shfl_up_sync(0xffffffffu, end, o);
+          const uint32_t y = __shfl_up_sync(0xffffffffu, end, o);
           if (lane >= o) end += y;
         }
         end += before;
@@ -329,60 +401,38 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int l = __ffs(hit) - 1;
           w.b = b0 + l;
           w.off = w0 - (__shfl_sync(0xffffffffu, end, l) - __shfl_sync(0xffffffffu, u, l));
+          w.s = make_seq(a, __shfl_sync(0xffffffffu, base, l), __shfl_sync(0xffffffffu, count, l), per_item);
           break;
         }
         before = __shfl_sync(0xffffffffu, end, 31);
       }
       w.left = int(min(chunk, total - w0));
     }
-    if (lane == 0) {
-      s_walk = w;
-      Meta m{0, 0, 0, 0, 0, int(chunk), {0, 0}};
-      Walk w2 = w;
-      Seg g;
-      if (next_seg(a, per_item, w2, g)) {
-        m.b = g.b;
-        m.kvh = g.kvh;
-        m.pair = g.pair;
-        m.j0 = g.j0;
-        m.nt = g.s.nt;
-      }
-      a.meta[blockIdx.x] = m;
-    }
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
-  auto fail = [&]() { atomicExch(&s_fail, 1); };
-  auto failed = [&]() { return *reinterpret_cast<volatile int*>(&s_fail) != 0; };
-
-  // Every role walks the same segments and counts ring loads, S tiles and
-  // segments for itself, so each barrier's phase is known without any
-  // block-wide synchronisation.  Ring loads of a segment of n tiles that
-  // starts at load c0:  K_0: c0;  K_j: c0 + 2j - 1;  V_j: c0 + 2j + 2, the last one c0 + 2n - 1.
-  Walk walk = s_walk;
-  Seg g;
-  if (warp == 0) {
-    // ---- TMA -------------------------------------------------------------------
     int nl = 0, si = 0;
     bool ok = true;
     const int br = a.kp.paged() ? min(a.kp.page_size, kTile) : kTile;  // rows per box
     const int nbox = kTile / br;
-    while (ok && next_seg(a, per_item, walk, g)) {
+    Seg g;
+    Meta m{0, 0, 0, 0, 0, 0, int(chunk), 0};
+    if (w.left == 0 && lane == 0) {  // nothing to do: an empty segment ends every role
+      s_seg[0] = Seg{Seq{}, 0, 0, 0, 0, 0, 1};
+      mbar_arrive(&seg_full[0]);
+    }
+    while (ok && next_seg(a, per_item, w, g)) {
       if (__any_sync(0xffffffffu, failed())) break;
-      const int qb = Wide ? 0 : si & 1, use = Wide ? si : si >> 1;
       if (lane == 0) {
-        if (use >= 1 && !mbar_wait(&q_empty[qb], (use - 1) & 1)) ok = false;
+        if (si >= 1 && !mbar_wait(q_empty, (si - 1) & 1)) ok = false;
         if (ok) {
+          s_seg[si % kSegs] = g;
+          mbar_arrive(&seg_full[si % kSegs]);
           const int t0 = g.pair * per_item;
           const bool second = Wide && t0 + a.tpt < g.s.count;
           const uint32_t bytes = uint32_t(L::kKB * a.tpt * a.group * 128);
-          mbar_expect_tx(&q_full[qb], second ? 2 * bytes : bytes);
+          mbar_expect_tx(q_full, second ? 2 * bytes : bytes);
           for (int t = 0; t < (second ? 2 : 1); ++t)
             for (int kb = 0; kb < L::kKB; ++kb)
-              tma_load_3d(smem + L::kQ + (Wide ? t : qb) * L::kBytesTile + kb * 16384, &qmap, &q_full[qb], kb * 64,
-                          g.kvh * a.group, g.b * a.tokens + t0 + t * a.tpt);
+              tma_load_3d(smem + L::kQ + t * L::kBytesTile + kb * 16384, &qmap, q_full, kb * 64, g.kvh * a.group,
+                          g.b * a.tokens + t0 + t * a.tpt);
         }
       }
       ok = __shfl_sync(0xffffffffu, ok, 0);
@@ -425,14 +475,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (ok) load(j, row, true);
         row = row1;
       }
+      if (si == 0) {
+        m.b = g.b;
+        m.kvh = g.kvh;
+        m.pair = g.pair;
+        m.count = g.s.count;
+        m.j0 = g.j0;
+        m.nt = g.s.nt;
+      }
       ++si;
     }
     if (!ok) fail();
-    // Let the loads in flight land before the block can end.
     if (lane == 0) {
+      a.meta[blockIdx.x] = m;
+      // Let the loads in flight land before the block can end.
       for (int c = max(0, nl - kNS); c < nl; ++c) mbar_wait(&full[c % kNS], (c / kNS) & 1);
-      for (int s = max(0, si - (Wide ? 1 : 2)); s < si; ++s)
-        mbar_wait(&q_full[Wide ? 0 : s & 1], (Wide ? s : s >> 1) & 1);
+      if (si > 0) mbar_wait(q_full, (si - 1) & 1);
     }
   } else if (warp == 1) {
     // ---- products (lane 0 issues; the warp waits and cleans V) -------------------
@@ -444,6 +502,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto slot_of = [&](int c) { return smem + L::kRing + (c % kNS) * L::kBytesTile; };
     auto release = [&](int c) {
       if (lane == 0) umma_commit(&empty[c % kNS]);
+      __syncwarp();
+    };
+    auto release_q = [&]() {
+      if (lane == 0) umma_commit(q_empty);
       __syncwarp();
     };
     auto issue_s = [&](int t, const uint8_t* q, const uint8_t* k) {
@@ -460,19 +522,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       __syncwarp();
     };
-    while (ok && next_seg(a, per_item, walk, g)) {
-      if (__any_sync(0xffffffffu, failed())) break;
+    const uint8_t* q0 = smem + L::kQ;
+    for (;;) {
+      if (!(ok = __all_sync(0xffffffffu, wait_seg(si)))) break;
+      const Seg g = s_seg[si % kSegs];
       const int n = g.j1 - g.j0;
-      const int qb = Wide ? 0 : si & 1, use = Wide ? si : si >> 1;
+      if (n == 0) break;
       const bool second = Wide ? g.pair * per_item + a.tpt < g.s.count : n > 1;  // the second group has work
-      const uint8_t* q0 = smem + L::kQ + qb * L::kBytesTile;
       auto k_load = [&](int i) { return i == 0 ? c0 : c0 + 2 * i - 1; };
       auto v_load = [&](int i) { return i == n - 1 ? c0 + 2 * n - 1 : c0 + 2 * i + 2; };
-      auto release_q = [&]() {
-        if (lane == 0) umma_commit(&q_empty[qb]);
-        __syncwarp();
-      };
-      if (!(ok = mbar_wait_warp(&q_full[qb], use & 1) && wait_load(k_load(0)))) break;
+      if (!(ok = mbar_wait_warp(q_full, si & 1) && wait_load(k_load(0)))) break;
       issue_s(0, q0, slot_of(k_load(0)));
       if constexpr (Wide) {
         if (second) issue_s(1, q0 + L::kBytesTile, slot_of(k_load(0)));
@@ -492,38 +551,42 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!(ok = wait_load(v_load(i)))) break;
         int node0;
         const int nv = tile_valid(g.s, g.j0 + i, node0), nv16 = (nv + 15) & ~15;
-        bool dirty = false;
-        // Rows past the tile's end, up to the last 16-row step of the product.
-        for (int e = lane; e < (nv16 - nv) * L::kKB * 8; e += 32) {
-          const int piece = e & 7, kb = (e >> 3) % L::kKB, r = nv + (e >> 3) / L::kKB;
-          *reinterpret_cast<uint4*>(v + kb * 16384 + r * 128 + piece * 16) = make_uint4(0, 0, 0, 0);
-          dirty = true;
-        }
-        if (node0 >= 0) {
-          bool odd = false;
-          for (int e = lane; e < nv * L::kKB * 8; e += 32) {  // the swizzle only permutes a row's pieces
-            const int piece = e & 7, kb = (e >> 3) % L::kKB, r = (e >> 3) / L::kKB;
-            uint4* p = reinterpret_cast<uint4*>(v + kb * 16384 + r * 128 + piece * 16);
-            const uint4 x = *p;
-            const uint4 y = make_uint4(split_finite(x.x, false), split_finite(x.y, false), split_finite(x.z, false),
-                                       split_finite(x.w, false));
-            if (x.x != y.x || x.y != y.y || x.z != y.z || x.w != y.w) {
-              *p = y;
-              odd = true;
-            }
-          }
-          if (__any_sync(0xffffffffu, odd)) {
+        if (nv < kTile || node0 >= 0) {
+          bool dirty = false;
+          // Rows past the tile's end, up to the last 16-row step of the product.
+          for (int e = lane; e < (nv16 - nv) * L::kKB * 8; e += 32) {
+            const int piece = e & 7, kb = (e >> 3) % L::kKB, r = nv + (e >> 3) / L::kKB;
+            *reinterpret_cast<uint4*>(v + kb * 16384 + r * 128 + piece * 16) = make_uint4(0, 0, 0, 0);
             dirty = true;
-            if (lane == 0) {
-              *reinterpret_cast<volatile int*>(&s_odd[si & 3]) = si + 1;
-              __threadfence_block();
+          }
+          if (node0 >= 0) {
+            bool odd = false;
+            for (int e = lane; e < nv * L::kKB * 8; e += 32) {  // the swizzle only permutes a row's pieces
+              const int piece = e & 7, kb = (e >> 3) % L::kKB, r = (e >> 3) / L::kKB;
+              uint4* p = reinterpret_cast<uint4*>(v + kb * 16384 + r * 128 + piece * 16);
+              const uint4 x = *p;
+              const uint4 y = make_uint4(split_finite(x.x, false), split_finite(x.y, false), split_finite(x.z, false),
+                                         split_finite(x.w, false));
+              if (x.x != y.x || x.y != y.y || x.z != y.z || x.w != y.w) {
+                *p = y;
+                odd = true;
+              }
+            }
+            if (__any_sync(0xffffffffu, odd)) {
+              dirty = true;
+              if (lane == 0) {
+                *reinterpret_cast<volatile int*>(&s_odd[si & 3]) = si + 1;
+                __threadfence_block();
+              }
             }
           }
+          if (__any_sync(0xffffffffu, dirty)) {
+            fence_proxy_async();
+            __syncwarp();
+          }
         }
-        if (__any_sync(0xffffffffu, dirty)) {
-          fence_proxy_async();
-          __syncwarp();
-        }
+        // O of the segment before must have been read before this one's first P V.
+        if (i == 0 && si >= 1 && !(ok = mbar_wait_warp(o_free, (si - 1) & 1))) break;
         const uint64_t vd = sw128_desc_mn(v, 16384);
         auto issue_o = [&](int t, bool first, bool last) {
           tc_fence_after();
@@ -564,228 +627,230 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) break;
       c0 += 2 * n;
       ++si;
+      if (g.last) break;
     }
     if (!ok) fail();
     if (lane == 0) umma_commit(mma_done);
     __syncwarp();
     mbar_wait_warp(mma_done, 0);
-  } else {
-    // ---- softmax and output: thread = query row ------------------------------------
+  } else if (warp < 4) {
     append_rows<D>(a, int(threadIdx.x) - 64);
-    const int t = (warp - 2) >> 2;  // group
+  } else {
+    // ---- softmax and output: two threads per query row --------------------------------
+    const int t = (warp - 4) >> 3, half = ((warp - 4) >> 2) & 1;
     const int quarter = warp & 3, row = quarter * 32 + lane;
+    const int pair_bar = 1 + t * 4 + quarter;  // shared with the warp of the other half
     const uint32_t lane_addr = uint32_t(quarter * 32) << 16;
     const uint32_t tS = tmem + lane_addr + uint32_t(t * 128);
     const uint32_t tO = tmem + lane_addr + L::kOCol;
     const float sl = kLog2e / sqrtf(float(D));
     const int node = row / a.group, head = row % a.group;
-    int ns = 0, si = 0, no[2] = {0, 0};  // S tiles, segments and finished O's so far
-    while (next_seg(a, per_item, walk, g)) {
-      if (__any_sync(0xffffffffu, failed())) break;
+    int ns = 0, no[2] = {0, 0};  // S tiles and finished O's so far
+    // After a wait that ran out nothing waits any more and nothing is written,
+    // but every step is still taken, so that the pairs' barriers stay complete.
+    bool ok = true;
+    for (int si = 0;; ++si) {
+      if (failed()) ok = false;
+      if (ok && !wait_seg(si)) ok = false;
+      ok = !pair_any(pair_bar, !ok);
+      if (!ok) {  // the segments may not be there: all softmax warps leave here
+        fail();
+        break;
+      }
+      const Seg g = s_seg[si % kSegs];
       const int n = g.j1 - g.j0;
+      if (n == 0) break;
       const int tok = g.pair * per_item + (Wide ? t * a.tpt : 0) + node;  // this row's node
       const bool live = node < a.tpt && tok < g.s.count;
       const bool warp_live = __any_sync(0xffffffffu, live);
       const bool mine = !Wide || t == 0 || g.pair * per_item + a.tpt < g.s.count;
       const int64_t qrow = int64_t(g.b) * a.tokens + tok;
       float m_ref = -INFINITY, l = 0.0f;
-      bool ok = true;
       if (mine) {
-        // The loop stays converged: a lane whose wait ran out stops waiting and
-        // records the failure; no output is written then.
         for (int i = Wide ? 0 : t; i < n; i += Wide ? 1 : 2) {
           int node0;
-          const int nv = tile_valid(g.s, g.j0 + i, node0);
-          uint32_t seen[4] = {0, 0, 0, 0};
+          const int nv = tile_valid(g.s, g.j0 + i, node0) - half * kHalf;  // of this thread's positions
+          uint32_t seen[2] = {0, 0};
           if (node0 >= 0 && live) {
-#pragma unroll
-            for (int w = 0; w < 4; ++w)
-              if (node0 / 32 + w < a.words) seen[w] = a.mask[qrow * a.words + node0 / 32 + w];
+            const int w = node0 / 32 + half * 2;
+            if (w < a.words) seen[0] = a.mask[qrow * a.words + w];
+            if (w + 1 < a.words) seen[1] = a.mask[qrow * a.words + w + 1];
           }
           if (ok && !mbar_wait(&s_full[t], ns & 1)) ok = false;
           ++ns;
           __syncwarp();  // the poll may have split the warp; tcgen05.ld needs it whole
           tc_fence_after();
           if (warp_live) {
-            uint32_t r[kTile];
-            tmem_ld64(tS, r);
-            tmem_ld64(tS + 64, r + 64);
+            uint32_t r[kHalf];
+            tmem_ld64(tS + uint32_t(half * kHalf), r);
             if (node0 >= 0) {
 #pragma unroll
-              for (int e = 0; e < kTile; ++e)
+              for (int e = 0; e < kHalf; ++e)
                 if (!(seen[e / 32] >> (e % 32) & 1) || e >= nv) r[e] = 0xFF800000u;
-            } else if (nv < kTile) {
+            } else if (nv < kHalf) {
 #pragma unroll
-              for (int e = 0; e < kTile; ++e)
+              for (int e = 0; e < kHalf; ++e)
                 if (e >= nv) r[e] = 0xFF800000u;
             }
-            // Row maximum of the raw scores, four independent chains; the scale is
+            // Maximum of the raw scores, four independent chains; the scale is
             // positive, so it is applied once to the maximum (base 2).
             float mc[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int e = 0; e < kTile; e += 8)
+            for (int e = 0; e < kHalf; e += 8)
 #pragma unroll
               for (int c = 0; c < 4; ++c)
                 mc[c] = fmax3(mc[c], __uint_as_float(r[e + 2 * c]), __uint_as_float(r[e + 2 * c + 1]));
-            const float mt = fmaxf(fmaxf(mc[0], mc[1]), fmaxf(mc[2], mc[3])) * sl;
-            bool rescale = false;
-            float corr = 1.0f;
-            if (mt > m_ref + kRescale) {  // also the first tile with anything to see (m_ref = -inf)
-              if (m_ref != -INFINITY) {
-                corr = ex2(m_ref - mt);
-                rescale = true;
+            float mt = fmaxf(fmaxf(mc[0], mc[1]), fmaxf(mc[2], mc[3])) * sl;
+            if (pair_any(pair_bar, mt > m_ref + kRescale)) {  // also the first tile with anything to see
+              // Both threads of a row take the larger maximum: exchanged in two
+              // columns of S, which both have read.
+              tmem_st1(tS + uint32_t(kHalf + half), __float_as_uint(mt));
+              tc_fence_before();
+              pair_sync(pair_bar);
+              tc_fence_after();
+              mt = fmaxf(mt, __uint_as_float(tmem_ld1(tS + uint32_t(kHalf + 1 - half))));
+              bool rescale = false;
+              float corr = 1.0f;
+              if (mt > m_ref + kRescale) {
+                if (m_ref != -INFINITY) {
+                  corr = ex2(m_ref - mt);
+                  rescale = true;
+                }
+                l *= corr;
+                m_ref = mt;
               }
-              l *= corr;
-              m_ref = mt;
+              // O is settled: its last P V completed before this S was published.
+              if (__any_sync(0xffffffffu, rescale)) {
+#pragma unroll 1
+                for (int c = 0; c < D / 2; c += 16) {
+                  uint32_t o16[16];
+                  const uint32_t at = tO + uint32_t(t * D + half * (D / 2) + c);
+                  tmem_ld16(at, o16);
+#pragma unroll
+                  for (int e = 0; e < 16; ++e) o16[e] = __float_as_uint(__uint_as_float(o16[e]) * corr);
+                  tmem_st16(at, o16);
+                }
+              }
             }
             // P = 2^(s sl - m_ref) as bf16 pairs, packed in place; -inf gives 0 (a row
-            // that sees nothing yet uses 0 for the maximum: no inf - inf).  bf16 by
+            // that sees nothing yet uses 0 for the reference: no inf - inf).  bf16 by
             // integer rounding: P is not negative, and this keeps the conversion off the
             // pipe that computes the exponentials.
             const float mneg = m_ref == -INFINITY ? 0.0f : -m_ref;
             const uint64_t sl2 = pack_f2(sl, sl), mneg2 = pack_f2(mneg, mneg);
-            uint64_t acc[4] = {0, 0, 0, 0};
+            uint64_t acc[2] = {0, 0};
 #pragma unroll
-            for (int e = 0; e < kTile; e += 2) {
+            for (int e = 0; e < kHalf; e += 2) {
               float x0, x1;
               unpack_f2(fma_f2(pack_f2(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), sl2, mneg2), x0, x1);
               x0 = ex2(x0);
               x1 = ex2(x1);
-              acc[(e >> 1) & 3] = add_f2(acc[(e >> 1) & 3], pack_f2(x0, x1));
+              acc[(e >> 1) & 1] = add_f2(acc[(e >> 1) & 1], pack_f2(x0, x1));
               r[e / 2] = __byte_perm(__float_as_uint(x0) + 0x8000u, __float_as_uint(x1) + 0x8000u, 0x7632);
             }
-            float a0, a1, a2, a3;
+            float a0, a1;
             unpack_f2(add_f2(acc[0], acc[1]), a0, a1);
-            unpack_f2(add_f2(acc[2], acc[3]), a2, a3);
-            l += (a0 + a1) + (a2 + a3);
-            // O is settled: its last P V completed before this S was published.
-            if (__any_sync(0xffffffffu, rescale)) {
-#pragma unroll
-              for (int c = 0; c < D / 32; ++c) {
-                uint32_t o32[32];
-                tmem_ld32(tO + uint32_t(t * D + c * 32), o32);
-#pragma unroll
-                for (int e = 0; e < 32; ++e) o32[e] = __float_as_uint(__uint_as_float(o32[e]) * corr);
-                tmem_st32(tO + uint32_t(t * D + c * 32), o32);
-              }
-            }
-            tmem_st64(tS, r);
+            l += a0 + a1;
+            tmem_st32p(tS + uint32_t(half * 32), r);
           }
           tc_fence_before();
-          __syncwarp();
-          // The first group reads O_1 of the segment before; until it has, the
-          // next P V must not start.
-          if (!Wide && t == 1 && i == 1 && si >= 1 && ok && !mbar_wait(o1_free, (si - 1) & 1)) ok = false;
           __syncwarp();
           if (lane == 0) mbar_arrive(&p_full[t]);
         }
       }
-      if (!Wide && t == 1) {
-        if (n < 2 && si >= 1 && ok && !mbar_wait(o1_free, (si - 1) & 1)) ok = false;
-        stat[row] = make_float2(m_ref, l);
-        if (!__all_sync(0xffffffffu, ok)) {
-          fail();
-          break;
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(st_full);
-        ++si;
-        continue;
-      }
-      if (mine) {
-        if (ok && !mbar_wait(&o_done[t], no[t] & 1)) ok = false;
-        ++no[t];
-      }
-      float w0 = 1.0f, w1 = 0.0f;  // weights of O_0 and O_1 (the first group joins both)
-      if (!Wide) {
-        if (n > 1) {
-          if (ok && !mbar_wait(&o_done[1], no[1] & 1)) ok = false;
-          ++no[1];
-        }
-        if (ok && !mbar_wait(st_full, si & 1)) ok = false;
-        __syncwarp();
-        if (n > 1) {
-          const float2 other = stat[row];
-          const float m = fmaxf(m_ref, other.x);
-          if (m != -INFINITY) {
-            w0 = ex2(m_ref - m);
-            w1 = ex2(other.x - m);
-          }
-          l = l * w0 + other.y * w1;
-          m_ref = m;
+      // ---- output ----------------------------------------------------------------------
+      // The statistics of the segment before have been read by everyone.
+      if (si >= 1 && ok && !mbar_wait(o_free, (si - 1) & 1)) ok = false;
+      s_sum[(t * 2 + half) * 128 + row] = l;
+      if (!Wide && half == 0) s_ref[t * 128 + row] = m_ref;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&st_full[t]);
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        if (Wide && x != t) continue;
+        if (ok && !mbar_wait(&st_full[x], si & 1)) ok = false;
+        if (Wide ? mine : x < n) {
+          if (ok && !mbar_wait(&o_done[x], no[x] & 1)) ok = false;
+          ++no[x];
         }
       }
       __syncwarp();
-      if (!__all_sync(0xffffffffu, ok)) {
-        fail();
-        break;
-      }
-      if (mine) {
-        tc_fence_after();
+      tc_fence_after();
+      if (mine && warp_live && __all_sync(0xffffffffu, ok)) {
+        float w0 = 1.0f, w1 = 0.0f;  // weights of O_0 and O_1 (not wide: both belong to the row)
+        l = s_sum[(t * 2) * 128 + row] + s_sum[(t * 2 + 1) * 128 + row];
+        if (!Wide) {
+          const float m0 = s_ref[row], m1 = n > 1 ? s_ref[128 + row] : -INFINITY;
+          const float l0 = s_sum[row] + s_sum[128 + row], l1 = s_sum[256 + row] + s_sum[384 + row];
+          m_ref = fmaxf(m0, m1);
+          w1 = n > 1 ? 1.0f : 0.0f;
+          if (m_ref != -INFINITY) {
+            w0 = ex2(m0 - m_ref);
+            w1 = ex2(m1 - m_ref);
+          }
+          l = l0 * w0 + l1 * w1;
+        }
         const bool whole = g.j0 == 0 && g.j1 == g.s.nt;
         const bool odd = *reinterpret_cast<volatile int*>(&s_odd[si & 3]) == si + 1;
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // a row that sees nothing: O is 0
         // A cut item: this part's place (0: the block's run starts in it).
-        const bool from_start = g.j0 != 0 || si == 0;
-        const int64_t slot = (int64_t(blockIdx.x) * 2 + (from_start ? 0 : 1)) * (Wide ? 2 : 1) + (Wide ? t : 0);
+        const int64_t slot = (int64_t(blockIdx.x) * 2 + (si == 0 ? 0 : 1)) * (Wide ? 2 : 1) + (Wide ? t : 0);
         float4* po = reinterpret_cast<float4*>(a.parts + slot * L::kPart);
         float2* pm = reinterpret_cast<float2*>(a.parts + slot * L::kPart + size_t(D / 4) * 128 * 16);
         uint16_t* orow = a.out + (qrow * a.heads + g.kvh * a.group + head) * D;
-        if (warp_live) {
+        constexpr int kCols = Wide ? D / 2 : D / 4;  // this thread's columns
+        const int col0 = (Wide ? half : t * 2 + half) * kCols;
+#pragma unroll 1
+        for (int c = col0; c < col0 + kCols; c += 16) {
+          float o[16];
+          {
+            uint32_t r[16];
+            tmem_ld16(tO + uint32_t((Wide ? t * D : 0) + c), r);
 #pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
-            float o[32];
-            {
-              uint32_t r[32];
-              tmem_ld32(tO + uint32_t((Wide ? t * D : 0) + c * 32), r);
+            for (int e = 0; e < 16; ++e) o[e] = __uint_as_float(r[e]);
+          }
+          if (!Wide && n > 1) {
+            uint32_t r[16];
+            tmem_ld16(tO + uint32_t(D + c), r);
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __uint_as_float(r[e]);
-            }
-            if (!Wide && n > 1) {
-              uint32_t r[32];
-              tmem_ld32(tO + uint32_t(D + c * 32), r);
+            for (int e = 0; e < 16; ++e) o[e] = o[e] * w0 + __uint_as_float(r[e]) * w1;
+          }
+          if (odd && live) {
+            for (int j = max(0, (g.j0 - g.s.prefix) * kTile); j < min(g.s.count, (g.j1 - g.s.prefix) * kTile); ++j) {
+              if (!(a.mask[qrow * a.words + j / 32] >> (j % 32) & 1)) continue;
+              const uint32_t* v = reinterpret_cast<const uint32_t*>(
+                  a.v_new + ((int64_t(g.b) * a.tokens + j) * a.kv_heads + g.kvh) * D + c);
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = o[e] * w0 + __uint_as_float(r[e]) * w1;
-            }
-            if (odd && live) {
-              for (int j = max(0, (g.j0 - g.s.prefix) * kTile); j < min(g.s.count, (g.j1 - g.s.prefix) * kTile); ++j) {
-                if (!(a.mask[qrow * a.words + j / 32] >> (j % 32) & 1)) continue;
-                const uint32_t* v = reinterpret_cast<const uint32_t*>(
-                    a.v_new + ((int64_t(g.b) * a.tokens + j) * a.kv_heads + g.kvh) * D + c * 32);
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                  const uint32_t x = split_finite(v[e], true);
-                  o[2 * e] += bf_lo(x);
-                  o[2 * e + 1] += bf_hi(x);
-                }
+              for (int e = 0; e < 8; ++e) {
+                const uint32_t x = split_finite(v[e], true);
+                o[2 * e] += bf_lo(x);
+                o[2 * e + 1] += bf_hi(x);
               }
-            }
-            if (live && whole) {
-#pragma unroll
-              for (int v = 0; v < 4; ++v) {
-                uint32_t w4[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w4[e] = pack_bf2(o[8 * v + 2 * e] * inv, o[8 * v + 2 * e + 1] * inv);
-                *reinterpret_cast<uint4*>(orow + c * 32 + 8 * v) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
-              }
-            } else if (live) {
-#pragma unroll
-              for (int v = 0; v < 8; ++v)
-                po[(c * 8 + v) * 128 + row] = make_float4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
             }
           }
-          if (live && !whole) pm[row] = make_float2(m_ref, l);
+          if (live && whole) {
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+              uint32_t w4[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) w4[e] = pack_bf2(o[8 * v + 2 * e] * inv, o[8 * v + 2 * e + 1] * inv);
+              *reinterpret_cast<uint4*>(orow + c + 8 * v) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
+            }
+          } else if (live) {
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+              po[(c / 4 + v) * 128 + row] = make_float4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
+          }
         }
-        // O has been read: the next segment's first P V may overwrite it (the
-        // arrival that lets it start is ordered after this fence).
-        tc_fence_before();
+        if (live && !whole && half == 0 && (Wide || t == 0)) pm[row] = make_float2(m_ref, l);
       }
-      if (!Wide) {
-        __syncwarp();
-        if (lane == 0) mbar_arrive(o1_free);
-      }
-      ++si;
+      // O and the statistics have been read.
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(o_free);
+      if (g.last) break;
     }
+    if (!ok) fail();
   }
   tc_fence_before();
   __syncthreads();
@@ -793,7 +858,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
   }
-  if (threadIdx.x == 0 && s_fail && a.err) atomicExch(a.err, 4);
+  if (threadIdx.x == 0 && *s_fail && a.err) atomicExch(a.err, 4);
 }
 
 // Joins the parts of the item that block c's run starts in the middle of, when
@@ -801,16 +866,15 @@ __global__ void __launch_bounds__(kThreads, 1)
 // columns of one query tile.
 template <int D, bool Wide>
 __global__ void __launch_bounds__(128) tree_join_kernel(const Args a) {
-  using L = Lay<D>;
+  using L = Lay<D, Wide>;
   pdl_trigger();
   pdl_wait();
   const int c = int(blockIdx.x), row = int(threadIdx.x);
   const int t = Wide ? int(blockIdx.y) / (D / 32) : 0, col = int(blockIdx.y) % (D / 32);
   const Meta m = a.meta[c];
   if (m.j0 == 0 || m.j0 > m.chunk) return;
-  const Seq s = seq_of(a, m.b, 1);
   const int tok = m.pair * a.tpt * (Wide ? 2 : 1) + t * a.tpt + row / a.group;
-  if (row / a.group >= a.tpt || tok >= s.count) return;
+  if (row / a.group >= a.tpt || tok >= m.count) return;
   const int parts = 2 + (m.nt - m.j0 - 1) / m.chunk;  // block c - 1's, then c, c + 1, ...
   auto place = [&](int k) {
     const int64_t slot = (int64_t(c - 1 + k) * 2 + (k == 0 && m.j0 < m.chunk ? 1 : 0)) * (Wide ? 2 : 1) + t;
@@ -853,7 +917,7 @@ constexpr size_t kMetaBytes = size_t(kNumSMs) * sizeof(Meta);
 
 template <int D, bool Wide>
 int launch(const TreeArgs& t, cudaStream_t st) {
-  using L = Lay<D>;
+  using L = Lay<D, Wide>;
   static PerDeviceOnce configured;
   if (!configured.run([] {
         return cudaFuncSetAttribute(tree_attention_kernel<D, Wide>, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -881,7 +945,9 @@ int launch(const TreeArgs& t, cudaStream_t st) {
   // A block per SM, fewer when there are not that many tiles even at full lengths.
   const int per_item = tpt * (Wide ? 2 : 1);
   const int64_t tiles = (t.max_len + kTile - 1) / kTile + (t.tokens + kTile - 1) / kTile;
-  const int64_t most = t.batch * t.kv_heads * ((t.tokens + per_item - 1) / per_item) * tiles;
+  const int64_t items = t.batch * t.kv_heads * ((t.tokens + per_item - 1) / per_item);
+  if (items > INT32_MAX / tiles) return SB_INVALID_ARGUMENT;
+  const int64_t most = items * tiles;
   const unsigned grid = unsigned(std::min<int64_t>(most, kNumSMs));
   if (launch_pdl(tree_attention_kernel<D, Wide>, dim3(grid), dim3(kThreads), size_t(L::kBytes), st, qm, km, vm, knm,
                  vnm, a) != cudaSuccess)
@@ -903,7 +969,7 @@ bool wide(int64_t tokens, int64_t heads, int64_t kv_heads) {
 }  // namespace
 
 uint64_t tree_attention_workspace_bytes(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim) {
-  const uint64_t part = head_dim == 128 ? Lay<128>::kPart : Lay<64>::kPart;
+  const uint64_t part = head_dim == 128 ? Lay<128, false>::kPart : Lay<64, false>::kPart;
   return kMetaBytes + uint64_t(kNumSMs) * 2 * part * (wide(tokens, heads, kv_heads) ? 2 : 1);
 }
 
