@@ -25,7 +25,7 @@
 // issues the products
 //   S = Q K^T    (A, B in shared memory; 128 x 128 f32 in TMEM)
 //   O += P V     (A = P in TMEM, written over S; B = the V tile as loaded)
-// warps 2 and 3 append the new rows, and warps 4-11 and 12-19 are two softmax
+// warp 2 appends the new rows, warp 3 cleans V tiles (below), and warps 4-11 and 12-19 are two softmax
 // groups: two threads per query row, 64 positions each.  With more than 128 rows
 // the two groups take a query tile each and share every KV tile; with up to 128
 // rows both work for the same query tile, one on the even and one on the odd KV
@@ -41,7 +41,8 @@
 // Masked places.  A masked score becomes -inf whatever it was.  0 * NaN must
 // not reach O either: V rows at or past a tile's end are zeroed in shared
 // memory, and so are non-finite values of a node's v; the rows that do see
-// such a node get its non-finite values added to their output.
+// such a node get its non-finite values added to their output.  Warp 3 does this
+// as soon as such a tile has arrived.
 //
 // Every wait is bounded; one that runs out sets error word 4 and the block
 // winds down (loads land, products finish, TMEM is freed).
@@ -91,7 +92,7 @@ struct Lay {
   static constexpr int kStat = kRing + kSlots * kBytesTile;  // sum [2 groups][2 halves][128], reference [2][128] (not wide)
   static constexpr int kSeg = kStat + 4 * 128 * 4 + (Wide ? 0 : 2 * 128 * 4);
   static constexpr int kBar = kSeg + kSegs * int(sizeof(Seg));
-  static constexpr int kBars = 2 * kSlots + 12 + kSegs;
+  static constexpr int kBars = 3 * kSlots + 12 + kSegs;
   static constexpr int kUse = kBar + kBars * 8 + 8 + 20;  // and the TMEM address, the failure word, four notes
   static constexpr int kBytes = kUse + 1024 < 232448 ? kUse + 1024 : 232448;
   static constexpr uint32_t kOCol = 256;
@@ -216,11 +217,18 @@ __device__ __forceinline__ uint32_t split_finite(uint32_t v, bool keep) {
   return (lo == keep ? v & 0xFFFFu : 0u) | (hi == keep ? v & 0xFFFF0000u : 0u);
 }
 
+__device__ __forceinline__ bool all_finite(uint32_t v) {
+  return (v & 0x7F80u) != 0x7F80u && (v & 0x7F800000u) != 0x7F800000u;
+}
+
+// Whether a V tile has rows past its end or nodes' rows.
+__device__ __forceinline__ bool needs_cleaning(int nv, int node0) { return nv < kTile || node0 >= 0; }
+
 // Appends the block's share of the new rows, and zeroes the output rows of
-// dead nodes.  Threads 0..63.
+// dead nodes.  One warp.
 template <int D>
 __device__ void append_rows(const Args& a, int tid) {
-  constexpr int kT = 64, kU = 4;  // threads; pieces in flight of each
+  constexpr int kT = 32, kU = 4;  // threads; pieces in flight of each
   constexpr int kPer = D / 8;  // 16-byte pieces per head
   const int rows = a.batch * a.tokens, pieces = a.kv_heads * kPer;
   for (int r = int(blockIdx.x); r < rows; r += int(gridDim.x)) {
@@ -292,9 +300,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     return;
   }
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBar);
-  uint64_t* full = bars;              // [kNS] ring slot loaded
+  uint64_t* full = bars;              // [kNS] ring slot loaded (and clean)
   uint64_t* empty = bars + kNS;       // [kNS] ring slot read by its products
-  uint64_t* seg_full = bars + 2 * kNS;  // [kSegs] segment written
+  uint64_t* raw = bars + 2 * kNS;     // [kNS] a V tile that warp 3 cleans first is loaded
+  uint64_t* seg_full = bars + 3 * kNS;  // [kSegs] segment written
   uint64_t* q_full = seg_full + kSegs;  // the segment's query tiles are loaded
   uint64_t* q_empty = q_full + 1;     // its S products are complete
   uint64_t* s_full = q_full + 2;      // [2] per group: S is in TMEM
@@ -318,6 +327,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int s = 0; s < kNS; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
+      mbar_init(&raw[s], 1);
     }
     for (int s = 0; s < kSegs; ++s) mbar_init(&seg_full[s], 1);
     mbar_init(q_full, 1);
@@ -449,9 +459,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       auto load = [&](int j, int row, bool is_v) {
         const int slot = nl % kNS, round = nl / kNS;
+        int node0;
+        const int nv = tile_valid(g.s, j, node0);
+        uint64_t* bar = is_v && needs_cleaning(nv, node0) ? &raw[slot] : &full[slot];
         if (lane == 0) {
           if (round >= 1 && !mbar_wait(&empty[slot], (round - 1) & 1)) ok = false;
-          if (ok) mbar_expect_tx(&full[slot], L::kBytesTile);
+          if (ok) mbar_expect_tx(bar, L::kBytesTile);
         }
         ok = __shfl_sync(0xffffffffu, ok, 0);
         if (!ok) return;
@@ -459,10 +472,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (j < g.s.prefix) {
           if (lane < nbox)
             for (int kb = 0; kb < L::kKB; ++kb)
-              tma_load_2d(dst + kb * 16384 + lane * br * 128, is_v ? &vmap : &kmap, &full[slot], kb * 64, row);
+              tma_load_2d(dst + kb * 16384 + lane * br * 128, is_v ? &vmap : &kmap, bar, kb * 64, row);
         } else if (lane == 0) {
           for (int kb = 0; kb < L::kKB; ++kb)
-            tma_load_2d(dst + kb * 16384, is_v ? &vnmap : &knmap, &full[slot], g.kvh * D + kb * 64,
+            tma_load_2d(dst + kb * 16384, is_v ? &vnmap : &knmap, bar, g.kvh * D + kb * 64,
                         g.b * a.tokens + (j - g.s.prefix) * kTile);
         }
         ++nl;
@@ -493,7 +506,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (si > 0) mbar_wait(q_full, (si - 1) & 1);
     }
   } else if (warp == 1) {
-    // ---- products (lane 0 issues; the warp waits and cleans V) -------------------
+    // ---- products (lane 0 issues; the warp waits) ---------------------------------
     constexpr uint32_t kIdS = idesc_bf16(kTile, kTile), kIdO = idesc_bf16(kTile, D, true);
     int c0 = 0, si = 0;
     int np[2] = {0, 0};  // P tiles of each group so far
@@ -551,40 +564,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!(ok = wait_load(v_load(i)))) break;
         int node0;
         const int nv = tile_valid(g.s, g.j0 + i, node0), nv16 = (nv + 15) & ~15;
-        if (nv < kTile || node0 >= 0) {
-          bool dirty = false;
-          // Rows past the tile's end, up to the last 16-row step of the product.
-          for (int e = lane; e < (nv16 - nv) * L::kKB * 8; e += 32) {
-            const int piece = e & 7, kb = (e >> 3) % L::kKB, r = nv + (e >> 3) / L::kKB;
-            *reinterpret_cast<uint4*>(v + kb * 16384 + r * 128 + piece * 16) = make_uint4(0, 0, 0, 0);
-            dirty = true;
-          }
-          if (node0 >= 0) {
-            bool odd = false;
-            for (int e = lane; e < nv * L::kKB * 8; e += 32) {  // the swizzle only permutes a row's pieces
-              const int piece = e & 7, kb = (e >> 3) % L::kKB, r = (e >> 3) / L::kKB;
-              uint4* p = reinterpret_cast<uint4*>(v + kb * 16384 + r * 128 + piece * 16);
-              const uint4 x = *p;
-              const uint4 y = make_uint4(split_finite(x.x, false), split_finite(x.y, false), split_finite(x.z, false),
-                                         split_finite(x.w, false));
-              if (x.x != y.x || x.y != y.y || x.z != y.z || x.w != y.w) {
-                *p = y;
-                odd = true;
-              }
-            }
-            if (__any_sync(0xffffffffu, odd)) {
-              dirty = true;
-              if (lane == 0) {
-                *reinterpret_cast<volatile int*>(&s_odd[si & 3]) = si + 1;
-                __threadfence_block();
-              }
-            }
-          }
-          if (__any_sync(0xffffffffu, dirty)) {
-            fence_proxy_async();
-            __syncwarp();
-          }
-        }
         // O of the segment before must have been read before this one's first P V.
         if (i == 0 && si >= 1 && !(ok = mbar_wait_warp(o_free, (si - 1) & 1))) break;
         const uint64_t vd = sw128_desc_mn(v, 16384);
@@ -633,8 +612,54 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) umma_commit(mma_done);
     __syncwarp();
     mbar_wait_warp(mma_done, 0);
-  } else if (warp < 4) {
-    append_rows<D>(a, int(threadIdx.x) - 64);
+  } else if (warp == 2) {
+    append_rows<D>(a, lane);
+  } else if (warp == 3) {
+    // ---- cleaning of V tiles ------------------------------------------------------------
+    // Such a tile's load signals raw[slot], and this warp signals full[slot].
+    int c0 = 0;
+    uint32_t parity = 0;  // of each slot's next such tile
+    bool ok = true;
+    for (int si = 0;; ++si) {
+      if (!(ok = __all_sync(0xffffffffu, wait_seg(si)))) break;
+      const Seg g = s_seg[si % kSegs];
+      const int n = g.j1 - g.j0;
+      for (int i = 0; i < n; ++i) {
+        int node0;
+        const int nv = tile_valid(g.s, g.j0 + i, node0), nv16 = (nv + 15) & ~15;
+        if (!needs_cleaning(nv, node0)) continue;
+        const int c = i == n - 1 ? c0 + 2 * n - 1 : c0 + 2 * i + 2, slot = c % kNS;
+        if (!(ok = mbar_wait_warp(&raw[slot], parity >> slot & 1))) break;
+        parity ^= 1u << slot;
+        uint8_t* v = smem + L::kRing + slot * L::kBytesTile;
+        // Rows past the tile's end, up to the last 16-row step of the product.
+        for (int e = lane; e < (nv16 - nv) * L::kKB * 8; e += 32) {
+          const int piece = e & 7, kb = (e >> 3) % L::kKB, r = nv + (e >> 3) / L::kKB;
+          *reinterpret_cast<uint4*>(v + kb * 16384 + r * 128 + piece * 16) = make_uint4(0, 0, 0, 0);
+        }
+        if (node0 >= 0) {
+          bool odd = false;
+          for (int e = lane; e < nv * L::kKB * 8; e += 32) {  // the swizzle only permutes a row's pieces
+            const int piece = e & 7, kb = (e >> 3) % L::kKB, r = (e >> 3) / L::kKB;
+            uint4* p = reinterpret_cast<uint4*>(v + kb * 16384 + r * 128 + piece * 16);
+            const uint4 x = *p;
+            if (!(all_finite(x.x) && all_finite(x.y) && all_finite(x.z) && all_finite(x.w))) {
+              *p = make_uint4(split_finite(x.x, false), split_finite(x.y, false), split_finite(x.z, false),
+                              split_finite(x.w, false));
+              odd = true;
+            }
+          }
+          if (__any_sync(0xffffffffu, odd) && lane == 0) *reinterpret_cast<volatile int*>(&s_odd[si & 3]) = si + 1;
+        }
+        __threadfence_block();
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[slot]);
+      }
+      if (!ok || n == 0 || g.last) break;
+      c0 += 2 * n;
+    }
+    if (!ok) fail();
   } else {
     // ---- softmax and output: two threads per query row --------------------------------
     const int t = (warp - 4) >> 3, half = ((warp - 4) >> 2) & 1;
@@ -862,55 +887,66 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // Joins the parts of the item that block c's run starts in the middle of, when
-// c is the first block whose run does.  Thread = query row, blockIdx.y = 32
-// columns of one query tile.
+// c is the first block whose run does.  Thread = query row, blockIdx.y = 8
+// columns of one query tile; parts are taken four at a time, all their loads in
+// flight together.
+constexpr int kJoinParts = 4;
 template <int D, bool Wide>
 __global__ void __launch_bounds__(128) tree_join_kernel(const Args a) {
   using L = Lay<D, Wide>;
   pdl_trigger();
   pdl_wait();
   const int c = int(blockIdx.x), row = int(threadIdx.x);
-  const int t = Wide ? int(blockIdx.y) / (D / 32) : 0, col = int(blockIdx.y) % (D / 32);
+  const int t = Wide ? int(blockIdx.y) / (D / 8) : 0, col = int(blockIdx.y) % (D / 8);
   const Meta m = a.meta[c];
   if (m.j0 == 0 || m.j0 > m.chunk) return;
   const int tok = m.pair * a.tpt * (Wide ? 2 : 1) + t * a.tpt + row / a.group;
   if (row / a.group >= a.tpt || tok >= m.count) return;
   const int parts = 2 + (m.nt - m.j0 - 1) / m.chunk;  // block c - 1's, then c, c + 1, ...
-  auto place = [&](int k) {
-    const int64_t slot = (int64_t(c - 1 + k) * 2 + (k == 0 && m.j0 < m.chunk ? 1 : 0)) * (Wide ? 2 : 1) + t;
-    return a.parts + slot * L::kPart;
-  };
-  float best = -INFINITY;
-  for (int k = 0; k < parts; ++k)
-    best = fmaxf(best, reinterpret_cast<const float2*>(place(k) + size_t(D / 4) * 128 * 16)[row].x);
-  float l = 0.0f, o[32];
+  float best = -INFINITY, l = 0.0f, o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  for (int k0 = 0; k0 < parts; k0 += kJoinParts) {
+    float2 ml[kJoinParts];
+    float4 x[kJoinParts][2];
 #pragma unroll
-  for (int e = 0; e < 32; ++e) o[e] = 0.0f;
-  for (int k = 0; k < parts; ++k) {
-    const uint8_t* p = place(k);
-    const float2 ml = reinterpret_cast<const float2*>(p + size_t(D / 4) * 128 * 16)[row];
-    // A part that sees nothing has O = 0, or a non-finite node's value.
-    const float w = best == -INFINITY || ml.x == best ? 1.0f : ex2(ml.x - best);
-    l += w * ml.y;
-    const float4* po = reinterpret_cast<const float4*>(p) + col * 8 * 128 + row;
-#pragma unroll
-    for (int v = 0; v < 8; ++v) {
-      const float4 x = po[v * 128];
-      o[4 * v] += w * x.x;
-      o[4 * v + 1] += w * x.y;
-      o[4 * v + 2] += w * x.z;
-      o[4 * v + 3] += w * x.w;
+    for (int q = 0; q < kJoinParts; ++q) {
+      const int k = k0 + q;
+      ml[q] = make_float2(-INFINITY, 0.0f);
+      x[q][0] = x[q][1] = make_float4(0, 0, 0, 0);
+      if (k < parts) {
+        const int64_t slot = (int64_t(c - 1 + k) * 2 + (k == 0 && m.j0 < m.chunk ? 1 : 0)) * (Wide ? 2 : 1) + t;
+        const uint8_t* p = a.parts + slot * L::kPart;
+        ml[q] = reinterpret_cast<const float2*>(p + size_t(D / 4) * 128 * 16)[row];
+        x[q][0] = reinterpret_cast<const float4*>(p)[(col * 2) * 128 + row];
+        x[q][1] = reinterpret_cast<const float4*>(p)[(col * 2 + 1) * 128 + row];
+      }
     }
+    float top = best;
+#pragma unroll
+    for (int q = 0; q < kJoinParts; ++q) top = fmaxf(top, ml[q].x);
+    // Nothing seen so far: every O is 0, or a non-finite node's value.
+    const float w0 = best == top ? 1.0f : ex2(best - top);
+    l *= w0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] *= w0;
+#pragma unroll
+    for (int q = 0; q < kJoinParts; ++q) {
+      const float w = ml[q].x == top ? 1.0f : ex2(ml[q].x - top);
+      l += w * ml[q].y;
+      o[0] += w * x[q][0].x;
+      o[1] += w * x[q][0].y;
+      o[2] += w * x[q][0].z;
+      o[3] += w * x[q][0].w;
+      o[4] += w * x[q][1].x;
+      o[5] += w * x[q][1].y;
+      o[6] += w * x[q][1].z;
+      o[7] += w * x[q][1].w;
+    }
+    best = top;
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  uint16_t* orow = a.out + ((int64_t(m.b) * a.tokens + tok) * a.heads + m.kvh * a.group + row % a.group) * D + col * 32;
-#pragma unroll
-  for (int v = 0; v < 4; ++v) {
-    uint32_t w4[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) w4[e] = pack_bf2(o[8 * v + 2 * e] * inv, o[8 * v + 2 * e + 1] * inv);
-    *reinterpret_cast<uint4*>(orow + 8 * v) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
-  }
+  uint16_t* orow = a.out + ((int64_t(m.b) * a.tokens + tok) * a.heads + m.kvh * a.group + row % a.group) * D + col * 8;
+  *reinterpret_cast<uint4*>(orow) = make_uint4(pack_bf2(o[0] * inv, o[1] * inv), pack_bf2(o[2] * inv, o[3] * inv),
+                                               pack_bf2(o[4] * inv, o[5] * inv), pack_bf2(o[6] * inv, o[7] * inv));
 }
 
 constexpr size_t kMetaBytes = size_t(kNumSMs) * sizeof(Meta);
@@ -954,7 +990,7 @@ int launch(const TreeArgs& t, cudaStream_t st) {
     return SB_INTERNAL;
   count_launch();
   if (grid == 1) return SB_OK;  // nothing is cut
-  if (launch_pdl(tree_join_kernel<D, Wide>, dim3(grid, unsigned(D / 32 * (Wide ? 2 : 1))), dim3(128), 0, st, a) !=
+  if (launch_pdl(tree_join_kernel<D, Wide>, dim3(grid, unsigned(D / 8 * (Wide ? 2 : 1))), dim3(128), 0, st, a) !=
       cudaSuccess)
     return SB_INTERNAL;
   count_launch();
