@@ -170,6 +170,27 @@ __device__ __forceinline__ bool next_seg(const Args& a, int per_item, Walk& w, S
   return true;
 }
 
+// Bounded wait for the phase with parity `parity` (mbar_wait, kept small: it
+// stands at two dozen places).
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity) {
+  const uint32_t at = su32(bar);
+#pragma unroll 1
+  for (uint32_t i = 0; i < kWaitLimit; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(done)
+        : "r"(at), "r"(parity)
+        : "memory");
+    if (done) return true;
+  }
+  return false;
+}
+// The same with one answer for the whole warp.
+__device__ __forceinline__ bool wait_bar_warp(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, wait_bar(bar, parity));
+}
+
 // Tile j of a segment: valid positions, and for a tile of nodes the first node (-1 for cached positions).
 __device__ __forceinline__ int tile_valid(const Seq& s, int j, int& node0) {
   if (j < s.prefix) {
@@ -178,6 +199,11 @@ __device__ __forceinline__ int tile_valid(const Seq& s, int j, int& node0) {
   }
   node0 = (j - s.prefix) * kTile;
   return min(kTile, s.count - node0);
+}
+
+// The n lowest bits (none for n <= 0, all for n >= 32).
+__device__ __forceinline__ uint32_t low_bits(int n) {
+  return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
 }
 
 // 2^x by the hardware approximation (relative error about 2^-22).
@@ -231,6 +257,7 @@ __device__ void append_rows(const Args& a, int tid) {
   constexpr int kT = 32, kU = 4;  // threads; pieces in flight of each
   constexpr int kPer = D / 8;  // 16-byte pieces per head
   const int rows = a.batch * a.tokens, pieces = a.kv_heads * kPer;
+#pragma unroll 1
   for (int r = int(blockIdx.x); r < rows; r += int(gridDim.x)) {
     const int b = r / a.tokens, t = r % a.tokens;
     bool bad;
@@ -238,6 +265,7 @@ __device__ void append_rows(const Args& a, int tid) {
     if (bad && t == 0 && tid == 0 && a.err) atomicExch(a.err, kBadPosition);
     if (t >= s.count) {
       uint4* o = reinterpret_cast<uint4*>(a.out) + int64_t(r) * a.heads * kPer;
+#pragma unroll 1
       for (int i = tid; i < a.heads * kPer; i += kT) o[i] = make_uint4(0, 0, 0, 0);
       continue;
     }
@@ -249,6 +277,7 @@ __device__ void append_rows(const Args& a, int tid) {
       continue;
     }
     const int64_t step = a.kp.paged() ? a.kp.page_size : a.max_len;  // rows between kv heads
+#pragma unroll 1
     for (int i0 = tid; i0 < pieces; i0 += kT * kU) {
       uint4 k[kU], v[kU];
 #pragma unroll
@@ -371,34 +400,24 @@ __global__ void __launch_bounds__(kThreads, 1)
   // one c0 + 2n - 1.  A segment's slot is written again four segments later:
   // then warp 0 has waited for the S products of two segments later, before
   // which warp 1 has waited for every softmax warp to be done with this one.
-  auto wait_seg = [&](int si) { return mbar_wait(&seg_full[si % kSegs], (si / kSegs) & 1); };
+  auto wait_seg = [&](int si) { return wait_bar(&seg_full[si % kSegs], (si / kSegs) & 1); };
   if (warp == 0) {
     // ---- the walk and the loads --------------------------------------------------
     // All tiles in one line, an equal run of it per block.
-    const int step = 32;
-    uint32_t total = 0;
-    int base = 0, count = 0;
-    auto units_of = [&](int b) {
-      base = count = 0;
-      if (b < a.batch) {
-        base = a.base[b];
-        count = a.count ? a.count[b] : a.tokens;
-      }
-      const Seq s = make_seq(a, base, count, per_item);
-      return uint32_t(s.nt) * uint32_t(a.kv_heads) * uint32_t(s.pairs);
-    };
-    uint32_t u = 0;
-    for (int b0 = 0; b0 < a.batch; b0 += step) {
-      u = units_of(b0 + lane);
-      total += __reduce_add_sync(0xffffffffu, u);
-    }
-    const uint32_t chunk = (total + gridDim.x - 1) / gridDim.x;
-    const uint32_t w0 = chunk * blockIdx.x;
+    uint32_t total = 0, chunk = 0, w0 = 0;
     Walk w{Seq{}, a.batch, 0, 0};
-    if (w0 < total) {
+#pragma unroll 1
+    for (int pass = 0; pass < 2; ++pass) {  // the sum of all tiles; then where this block's run starts
       uint32_t before = 0;
-      for (int b0 = 0; b0 < a.batch; b0 += step) {
-        if (a.batch > step) u = units_of(b0 + lane);
+#pragma unroll 1
+      for (int b0 = 0; b0 < a.batch; b0 += 32) {
+        int base = 0, count = 0;
+        if (b0 + lane < a.batch) {
+          base = a.base[b0 + lane];
+          count = a.count ? a.count[b0 + lane] : a.tokens;
+        }
+        const Seq s = make_seq(a, base, count, per_item);
+        const uint32_t u = uint32_t(s.nt) * uint32_t(a.kv_heads) * uint32_t(s.pairs);
         uint32_t end = u;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -406,17 +425,25 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (lane >= o) end += y;
         }
         end += before;
-        const uint32_t hit = __ballot_sync(0xffffffffu, w0 < end);
-        if (hit) {
-          const int l = __ffs(hit) - 1;
-          w.b = b0 + l;
-          w.off = w0 - (__shfl_sync(0xffffffffu, end, l) - __shfl_sync(0xffffffffu, u, l));
-          w.s = make_seq(a, __shfl_sync(0xffffffffu, base, l), __shfl_sync(0xffffffffu, count, l), per_item);
-          break;
-        }
         before = __shfl_sync(0xffffffffu, end, 31);
+        if (b0 + 32 >= a.batch && pass == 0) {
+          total = before;
+          chunk = (total + gridDim.x - 1) / gridDim.x;
+          w0 = chunk * blockIdx.x;
+        }
+        if ((pass == 1 || a.batch <= 32) && w0 < total) {
+          const uint32_t hit = __ballot_sync(0xffffffffu, w0 < end);
+          if (hit) {
+            const int l = __ffs(hit) - 1;
+            w.b = b0 + l;
+            w.off = w0 - (__shfl_sync(0xffffffffu, end, l) - __shfl_sync(0xffffffffu, u, l));
+            w.s = make_seq(a, __shfl_sync(0xffffffffu, base, l), __shfl_sync(0xffffffffu, count, l), per_item);
+            w.left = int(min(chunk, total - w0));
+            break;
+          }
+        }
       }
-      w.left = int(min(chunk, total - w0));
+      if (a.batch <= 32) break;
     }
     int nl = 0, si = 0;
     bool ok = true;
@@ -431,7 +458,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     while (ok && next_seg(a, per_item, w, g)) {
       if (__any_sync(0xffffffffu, failed())) break;
       if (lane == 0) {
-        if (si >= 1 && !mbar_wait(q_empty, (si - 1) & 1)) ok = false;
+        if (si >= 1 && !wait_bar(q_empty, (si - 1) & 1)) ok = false;
         if (ok) {
           s_seg[si % kSegs] = g;
           mbar_arrive(&seg_full[si % kSegs]);
@@ -463,7 +490,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int nv = tile_valid(g.s, j, node0);
         uint64_t* bar = is_v && needs_cleaning(nv, node0) ? &raw[slot] : &full[slot];
         if (lane == 0) {
-          if (round >= 1 && !mbar_wait(&empty[slot], (round - 1) & 1)) ok = false;
+          if (round >= 1 && !wait_bar(&empty[slot], (round - 1) & 1)) ok = false;
           if (ok) mbar_expect_tx(bar, L::kBytesTile);
         }
         ok = __shfl_sync(0xffffffffu, ok, 0);
@@ -480,13 +507,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         ++nl;
       };
-      int row = box_row(g.j0);
-      load(g.j0, row, false);
-      for (int j = g.j0; j < g.j1 && ok; ++j) {
-        const int row1 = j + 1 < g.j1 ? box_row(j + 1) : 0;
-        if (j + 1 < g.j1) load(j + 1, row1, false);
-        if (ok) load(j, row, true);
-        row = row1;
+      // K_0, then K_1, V_0, K_2, V_1, ..., and the last V: load i of the segment
+      // is the K tile (i + 1) / 2 for odd i (and i = 0), else the V tile i / 2 - 1.
+      // Map rows of the next V tile, the next K tile and the one after, so that the
+      // block table is read two tiles ahead.
+      const int n = g.j1 - g.j0;
+      int row = 0, next = box_row(g.j0), later = n > 1 ? box_row(g.j0 + 1) : 0;
+#pragma unroll 1
+      for (int i = 0; i < 2 * n && ok; ++i) {
+        const bool is_v = i == 2 * n - 1 || (i > 0 && !(i & 1));
+        const int j = g.j0 + (i == 2 * n - 1 ? n - 1 : is_v ? i / 2 - 1 : (i + 1) / 2);
+        load(j, is_v ? row : next, is_v);
+        if (is_v || i == 0) {  // the K tile loaded last is the next V tile
+          row = next;
+          next = later;
+          const int k = j + (is_v ? 3 : 2);
+          if (k < g.j1) later = box_row(k);
+        }
       }
       if (si == 0) {
         m.b = g.b;
@@ -502,8 +539,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       a.meta[blockIdx.x] = m;
       // Let the loads in flight land before the block can end.
-      for (int c = max(0, nl - kNS); c < nl; ++c) mbar_wait(&full[c % kNS], (c / kNS) & 1);
-      if (si > 0) mbar_wait(q_full, (si - 1) & 1);
+      for (int c = max(0, nl - kNS); c < nl; ++c) wait_bar(&full[c % kNS], (c / kNS) & 1);
+      if (si > 0) wait_bar(q_full, (si - 1) & 1);
     }
   } else if (warp == 1) {
     // ---- products (lane 0 issues; the warp waits) ---------------------------------
@@ -511,7 +548,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int c0 = 0, si = 0;
     int np[2] = {0, 0};  // P tiles of each group so far
     bool ok = true;
-    auto wait_load = [&](int c) { return mbar_wait_warp(&full[c % kNS], (c / kNS) & 1); };
+    auto wait_load = [&](int c) { return wait_bar_warp(&full[c % kNS], (c / kNS) & 1); };
     auto slot_of = [&](int c) { return smem + L::kRing + (c % kNS) * L::kBytesTile; };
     auto release = [&](int c) {
       if (lane == 0) umma_commit(&empty[c % kNS]);
@@ -544,7 +581,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool second = Wide ? g.pair * per_item + a.tpt < g.s.count : n > 1;  // the second group has work
       auto k_load = [&](int i) { return i == 0 ? c0 : c0 + 2 * i - 1; };
       auto v_load = [&](int i) { return i == n - 1 ? c0 + 2 * n - 1 : c0 + 2 * i + 2; };
-      if (!(ok = mbar_wait_warp(q_full, si & 1) && wait_load(k_load(0)))) break;
+      if (!(ok = wait_bar_warp(q_full, si & 1) && wait_load(k_load(0)))) break;
       issue_s(0, q0, slot_of(k_load(0)));
       if constexpr (Wide) {
         if (second) issue_s(1, q0 + L::kBytesTile, slot_of(k_load(0)));
@@ -565,14 +602,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         int node0;
         const int nv = tile_valid(g.s, g.j0 + i, node0), nv16 = (nv + 15) & ~15;
         // O of the segment before must have been read before this one's first P V.
-        if (i == 0 && si >= 1 && !(ok = mbar_wait_warp(o_free, (si - 1) & 1))) break;
+        if (i == 0 && si >= 1 && !(ok = wait_bar_warp(o_free, (si - 1) & 1))) break;
         const uint64_t vd = sw128_desc_mn(v, 16384);
         auto issue_o = [&](int t, bool first, bool last) {
           tc_fence_after();
           if (lane == 0) {
             const uint32_t tP = tmem + uint32_t(t * 128), tO = tmem + L::kOCol + uint32_t(t * D);
-            for (int kk = 0; kk < nv16 / 16; ++kk)
-              umma_bf16_ts(tO, tP + uint32_t(kk * 8), vd + uint64_t(kk * (2048 >> 4)), kIdO, !(first && kk == 0));
+#pragma unroll
+            for (int kk = 0; kk < kTile / 16; ++kk)
+              if (kk < nv16 / 16)
+                umma_bf16_ts(tO, tP + uint32_t(kk * 8), vd + uint64_t(kk * (2048 >> 4)), kIdO, !(first && kk == 0));
             if (last) umma_commit(&o_done[t]);
           }
           __syncwarp();
@@ -580,7 +619,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if constexpr (Wide) {
           if (i + 1 < n && !(ok = wait_load(k_load(i + 1)))) break;
           for (int t = 0; t < (second ? 2 : 1) && ok; ++t) {
-            if (!(ok = mbar_wait_warp(&p_full[t], np[t] & 1))) break;
+            if (!(ok = wait_bar_warp(&p_full[t], np[t] & 1))) break;
             ++np[t];
             issue_o(t, i == 0, i == n - 1);
             if (i + 1 < n) issue_s(t, q0 + t * L::kBytesTile, slot_of(k_load(i + 1)));
@@ -591,7 +630,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (i == n - 2) release_q();
         } else {
           const int t = i & 1;
-          if (!(ok = mbar_wait_warp(&p_full[t], np[t] & 1))) break;
+          if (!(ok = wait_bar_warp(&p_full[t], np[t] & 1))) break;
           ++np[t];
           issue_o(t, i < 2, i + 2 >= n);
           release(v_load(i));
@@ -611,7 +650,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (!ok) fail();
     if (lane == 0) umma_commit(mma_done);
     __syncwarp();
-    mbar_wait_warp(mma_done, 0);
+    wait_bar_warp(mma_done, 0);
   } else if (warp == 2) {
     append_rows<D>(a, lane);
   } else if (warp == 3) {
@@ -629,16 +668,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int nv = tile_valid(g.s, g.j0 + i, node0), nv16 = (nv + 15) & ~15;
         if (!needs_cleaning(nv, node0)) continue;
         const int c = i == n - 1 ? c0 + 2 * n - 1 : c0 + 2 * i + 2, slot = c % kNS;
-        if (!(ok = mbar_wait_warp(&raw[slot], parity >> slot & 1))) break;
+        if (!(ok = wait_bar_warp(&raw[slot], parity >> slot & 1))) break;
         parity ^= 1u << slot;
         uint8_t* v = smem + L::kRing + slot * L::kBytesTile;
         // Rows past the tile's end, up to the last 16-row step of the product.
+#pragma unroll 1
         for (int e = lane; e < (nv16 - nv) * L::kKB * 8; e += 32) {
           const int piece = e & 7, kb = (e >> 3) % L::kKB, r = nv + (e >> 3) / L::kKB;
           *reinterpret_cast<uint4*>(v + kb * 16384 + r * 128 + piece * 16) = make_uint4(0, 0, 0, 0);
         }
         if (node0 >= 0) {
           bool odd = false;
+#pragma unroll 2
           for (int e = lane; e < nv * L::kKB * 8; e += 32) {  // the swizzle only permutes a row's pieces
             const int piece = e & 7, kb = (e >> 3) % L::kKB, r = (e >> 3) / L::kKB;
             uint4* p = reinterpret_cast<uint4*>(v + kb * 16384 + r * 128 + piece * 16);
@@ -695,27 +736,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = Wide ? 0 : t; i < n; i += Wide ? 1 : 2) {
           int node0;
           const int nv = tile_valid(g.s, g.j0 + i, node0) - half * kHalf;  // of this thread's positions
-          uint32_t seen[2] = {0, 0};
-          if (node0 >= 0 && live) {
+          // The positions this row sees, of this thread's 64.
+          uint32_t seen[2] = {low_bits(nv), low_bits(nv - 32)};
+          if (node0 >= 0) {
             const int w = node0 / 32 + half * 2;
-            if (w < a.words) seen[0] = a.mask[qrow * a.words + w];
-            if (w + 1 < a.words) seen[1] = a.mask[qrow * a.words + w + 1];
+            seen[0] &= live && w < a.words ? a.mask[qrow * a.words + w] : 0u;
+            seen[1] &= live && w + 1 < a.words ? a.mask[qrow * a.words + w + 1] : 0u;
           }
-          if (ok && !mbar_wait(&s_full[t], ns & 1)) ok = false;
+          if (ok && !wait_bar(&s_full[t], ns & 1)) ok = false;
           ++ns;
           __syncwarp();  // the poll may have split the warp; tcgen05.ld needs it whole
           tc_fence_after();
           if (warp_live) {
             uint32_t r[kHalf];
             tmem_ld64(tS + uint32_t(half * kHalf), r);
-            if (node0 >= 0) {
+            if (node0 >= 0 || nv < kHalf) {
 #pragma unroll
               for (int e = 0; e < kHalf; ++e)
-                if (!(seen[e / 32] >> (e % 32) & 1) || e >= nv) r[e] = 0xFF800000u;
-            } else if (nv < kHalf) {
-#pragma unroll
-              for (int e = 0; e < kHalf; ++e)
-                if (e >= nv) r[e] = 0xFF800000u;
+                if (!(seen[e / 32] >> (e % 32) & 1)) r[e] = 0xFF800000u;
             }
             // Maximum of the raw scores, four independent chains; the scale is
             // positive, so it is applied once to the maximum (base 2).
@@ -785,7 +823,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       // ---- output ----------------------------------------------------------------------
       // The statistics of the segment before have been read by everyone.
-      if (si >= 1 && ok && !mbar_wait(o_free, (si - 1) & 1)) ok = false;
+      if (si >= 1 && ok && !wait_bar(o_free, (si - 1) & 1)) ok = false;
       s_sum[(t * 2 + half) * 128 + row] = l;
       if (!Wide && half == 0) s_ref[t * 128 + row] = m_ref;
       __syncwarp();
@@ -793,9 +831,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         if (Wide && x != t) continue;
-        if (ok && !mbar_wait(&st_full[x], si & 1)) ok = false;
+        if (ok && !wait_bar(&st_full[x], si & 1)) ok = false;
         if (Wide ? mine : x < n) {
-          if (ok && !mbar_wait(&o_done[x], no[x] & 1)) ok = false;
+          if (ok && !wait_bar(&o_done[x], no[x] & 1)) ok = false;
           ++no[x];
         }
       }
@@ -841,6 +879,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int e = 0; e < 16; ++e) o[e] = o[e] * w0 + __uint_as_float(r[e]) * w1;
           }
           if (odd && live) {
+#pragma unroll 1
             for (int j = max(0, (g.j0 - g.s.prefix) * kTile); j < min(g.s.count, (g.j1 - g.s.prefix) * kTile); ++j) {
               if (!(a.mask[qrow * a.words + j / 32] >> (j % 32) & 1)) continue;
               const uint32_t* v = reinterpret_cast<const uint32_t*>(
