@@ -69,17 +69,26 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, u
       : "memory");
 }
 
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z,
+                                            int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];" ::"r"(su32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(su32(bar))
+      : "memory");
+}
+
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
 
 // Shared-memory matrix descriptor of a K-major, 128-byte-swizzled tile whose
-// rows are 128 bytes (64 bf16): 8-row core groups 1024 bytes apart.
-__device__ __forceinline__ uint64_t sw128_desc(const void* tile) {
+// rows are 128 bytes (64 bf16): 8-row core groups `group_bytes` apart (1024: dense).
+__device__ __forceinline__ uint64_t sw128_desc(const void* tile, uint32_t group_bytes = 1024) {
   const uint32_t a = su32(tile);
   uint64_t d = uint64_t((a & 0x3FFFF) >> 4);  // start address
   d |= uint64_t(1) << 16;                      // leading byte offset (unused when swizzled)
-  d |= uint64_t(1024 >> 4) << 32;              // stride byte offset
+  d |= uint64_t(group_bytes >> 4) << 32;       // stride byte offset
   d |= uint64_t(1) << 46;                      // descriptor version
   d |= uint64_t(2) << 61;                      // SWIZZLE_128B
   return d;
@@ -87,13 +96,14 @@ __device__ __forceinline__ uint64_t sw128_desc(const void* tile) {
 
 // Shared-memory matrix descriptor of an MN-major, 128-byte-swizzled tile: 128-byte
 // rows of 64 consecutive M (or N) elements, one row per K index, 8-row groups
-// 1024 bytes apart (stride byte offset), and the next 64 M (or N) elements
+// `group_bytes` apart (stride byte offset), and the next 64 M (or N) elements
 // `mn_block_bytes` further on (leading byte offset).
-__device__ __forceinline__ uint64_t sw128_desc_mn(const void* tile, uint32_t mn_block_bytes) {
+__device__ __forceinline__ uint64_t sw128_desc_mn(const void* tile, uint32_t mn_block_bytes,
+                                                  uint32_t group_bytes = 1024) {
   const uint32_t a = su32(tile);
   uint64_t d = uint64_t((a & 0x3FFFF) >> 4);
   d |= uint64_t((mn_block_bytes >> 4) & 0x3FFF) << 16;
-  d |= uint64_t(1024 >> 4) << 32;
+  d |= uint64_t(group_bytes >> 4) << 32;
   d |= uint64_t(1) << 46;
   d |= uint64_t(2) << 61;
   return d;
@@ -281,17 +291,20 @@ inline bool make_map_2d(CUtensorMap* map, const void* base, CUtensorMapDataType 
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// A dense row-major 3-D tensor [d2, d1, d0] of bf16 as boxes of 64 x b1 x b2,
-// 128-byte swizzled.
-inline bool make_map_3d_bf16(CUtensorMap* map, const void* base, uint64_t d0, uint64_t d1, uint64_t d2, uint32_t b1,
-                             uint32_t b2) {
+// A bf16 tensor of up to four dimensions (fastest first; strides in elements
+// from the second on) as 128-byte-swizzled boxes.
+inline bool make_map_bf16(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
+                          const uint32_t* box) {
   EncodeTiledFn enc = encode_tiled_fn();
-  if (!enc) return false;
-  const cuuint64_t dims[3] = {d0, d1, d2};
-  const cuuint64_t strides[2] = {d0 * 2, d0 * d1 * 2};
-  const cuuint32_t box[3] = {64, b1, b2};
-  const cuuint32_t estr[3] = {1, 1, 1};
-  return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+  if (!enc || rank > 4) return false;
+  cuuint64_t d[4], st[4];
+  cuuint32_t bx[4], es[4] = {1, 1, 1, 1};
+  for (int i = 0; i < rank; ++i) {
+    d[i] = dims[i];
+    bx[i] = box[i];
+    if (i > 0) st[i - 1] = strides[i - 1] * 2;
+  }
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, cuuint32_t(rank), const_cast<void*>(base), d, st, bx, es,
              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }

@@ -85,7 +85,8 @@ struct Seg {
 template <int D, bool Wide>
 struct Lay {
   static constexpr int kKB = D / 64;              // 64-wide blocks of head_dim
-  static constexpr int kBytesTile = 128 * D * 2;  // kKB blocks of [128 rows][128 bytes]
+  static constexpr int kBytesTile = 128 * D * 2;  // a query tile: kKB blocks of [128 rows][128 bytes]
+  static constexpr int kGroup = kKB * 1024;       // a K or V tile: 16 groups of kKB blocks of [8 rows][128 bytes]
   static constexpr int kSlots = D == 128 ? 5 : 8;
   static constexpr int kQ = 0;
   static constexpr int kRing = (Wide ? 2 : 1) * kBytesTile;
@@ -119,6 +120,7 @@ struct Args {
   int words;       // mask words per node
   KvPages kp;
   int pool_rows;
+  int box_rows;  // rows of a K or V box: 8, or a multiple of 8 that a map of whole groups gives
   Meta* meta;
   uint8_t* parts;
   int* err;
@@ -447,8 +449,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     int nl = 0, si = 0;
     bool ok = true;
-    const int br = a.kp.paged() ? min(a.kp.page_size, kTile) : kTile;  // rows per box
-    const int nbox = kTile / br;
+    const int br = a.box_rows, nbox = kTile / br;
     Seg g;
     Meta m{0, 0, 0, 0, 0, 0, int(chunk), 0};
     if (w.left == 0 && lane == 0) {  // nothing to do: an empty segment ends every role
@@ -491,19 +492,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint64_t* bar = is_v && needs_cleaning(nv, node0) ? &raw[slot] : &full[slot];
         if (lane == 0) {
           if (round >= 1 && !wait_bar(&empty[slot], (round - 1) & 1)) ok = false;
-          if (ok) mbar_expect_tx(bar, L::kBytesTile);
+          // All of a cached tile; the 8-row groups of a tile of nodes that hold one.
+          if (ok) mbar_expect_tx(bar, j < g.s.prefix ? L::kBytesTile : (nv + 7) / 8 * L::kGroup);
         }
         ok = __shfl_sync(0xffffffffu, ok, 0);
         if (!ok) return;
         uint8_t* dst = smem + L::kRing + slot * L::kBytesTile;
         if (j < g.s.prefix) {
-          if (lane < nbox)
-            for (int kb = 0; kb < L::kKB; ++kb)
-              tma_load_2d(dst + kb * 16384 + lane * br * 128, is_v ? &vmap : &kmap, bar, kb * 64, row);
-        } else if (lane == 0) {
-          for (int kb = 0; kb < L::kKB; ++kb)
-            tma_load_2d(dst + kb * 16384, is_v ? &vnmap : &knmap, bar, g.kvh * D + kb * 64,
-                        g.b * a.tokens + (j - g.s.prefix) * kTile);
+          if (lane < nbox) {
+            uint8_t* at = dst + lane * (br / 8) * L::kGroup;
+            if (br > 8) tma_load_4d(at, is_v ? &vmap : &kmap, bar, 0, 0, 0, row / 8);
+            else tma_load_3d(at, is_v ? &vmap : &kmap, bar, 0, row, 0);
+          }
+        } else if (lane < (nv + 7) / 8) {
+          tma_load_4d(dst + lane * L::kGroup, is_v ? &vnmap : &knmap, bar, 0,
+                      g.b * a.tokens + (j - g.s.prefix) * kTile + lane * 8, 0, g.kvh);
         }
         ++nl;
       };
@@ -563,7 +566,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) {
 #pragma unroll
         for (int kb = 0; kb < L::kKB; ++kb) {
-          const uint64_t da = sw128_desc(q + kb * 16384), db = sw128_desc(k + kb * 16384);
+          const uint64_t da = sw128_desc(q + kb * 16384), db = sw128_desc(k + kb * 1024, L::kGroup);
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
             umma_bf16(tmem + uint32_t(t * 128), da + uint64_t(2 * kk), db + uint64_t(2 * kk), kIdS, (kb | kk) != 0);
@@ -603,7 +606,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int nv = tile_valid(g.s, g.j0 + i, node0), nv16 = (nv + 15) & ~15;
         // O of the segment before must have been read before this one's first P V.
         if (i == 0 && si >= 1 && !(ok = wait_bar_warp(o_free, (si - 1) & 1))) break;
-        const uint64_t vd = sw128_desc_mn(v, 16384);
+        const uint64_t vd = sw128_desc_mn(v, 1024, L::kGroup);
         auto issue_o = [&](int t, bool first, bool last) {
           tc_fence_after();
           if (lane == 0) {
@@ -611,7 +614,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int kk = 0; kk < kTile / 16; ++kk)
               if (kk < nv16 / 16)
-                umma_bf16_ts(tO, tP + uint32_t(kk * 8), vd + uint64_t(kk * (2048 >> 4)), kIdO, !(first && kk == 0));
+                umma_bf16_ts(tO, tP + uint32_t(kk * 8), vd + uint64_t(kk * (2 * L::kGroup >> 4)), kIdO, !(first && kk == 0));
             if (last) umma_commit(&o_done[t]);
           }
           __syncwarp();
@@ -675,14 +678,15 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
         for (int e = lane; e < (nv16 - nv) * L::kKB * 8; e += 32) {
           const int piece = e & 7, kb = (e >> 3) % L::kKB, r = nv + (e >> 3) / L::kKB;
-          *reinterpret_cast<uint4*>(v + kb * 16384 + r * 128 + piece * 16) = make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(v + (r / 8) * L::kGroup + kb * 1024 + (r % 8) * 128 + piece * 16) =
+              make_uint4(0, 0, 0, 0);
         }
         if (node0 >= 0) {
           bool odd = false;
 #pragma unroll 2
           for (int e = lane; e < nv * L::kKB * 8; e += 32) {  // the swizzle only permutes a row's pieces
             const int piece = e & 7, kb = (e >> 3) % L::kKB, r = (e >> 3) / L::kKB;
-            uint4* p = reinterpret_cast<uint4*>(v + kb * 16384 + r * 128 + piece * 16);
+            uint4* p = reinterpret_cast<uint4*>(v + (r / 8) * L::kGroup + kb * 1024 + (r % 8) * 128 + piece * 16);
             const uint4 x = *p;
             if (!(all_finite(x.x) && all_finite(x.y) && all_finite(x.z) && all_finite(x.w))) {
               *p = make_uint4(split_finite(x.x, false), split_finite(x.y, false), split_finite(x.z, false),
@@ -1004,18 +1008,38 @@ int launch(const TreeArgs& t, cudaStream_t st) {
   const uint64_t rows = uint64_t(t.batch) * uint64_t(t.tokens);
   const uint64_t kv_rows = paged ? uint64_t(t.kp.num_pages) * uint64_t(t.kv_heads) * uint64_t(t.kp.page_size)
                                  : uint64_t(t.batch) * uint64_t(t.kv_heads) * uint64_t(t.max_len);
-  const uint32_t box = paged ? uint32_t(std::min(t.kp.page_size, kTile)) : uint32_t(kTile);
-  auto map = [](CUtensorMap* m, const void* p, uint64_t r, uint64_t cols, uint32_t b) {
-    return make_map_2d(m, p, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, r, cols, 64, b, CU_TENSOR_MAP_SWIZZLE_128B);
+  // K and V tiles lie in shared memory as groups of 8 rows, a group's 64-wide
+  // blocks side by side, so that one box brings whole groups: a page, or a tile
+  // of a contiguous cache whose sequences start on 8 rows.  One box of 128 rows
+  // instead of two of 64 columns, and 8 instead of 16 for 16-row pages: 32 x 16
+  // nodes over 4096 positions in 16-row pages 149 -> 131 us.  Rows that start
+  // anywhere (the nodes' own, and other contiguous caches) come 8 at a time.
+  constexpr uint64_t kKB = D / 64;
+  const bool grouped = paged || t.max_len % 8 == 0;
+  const uint32_t box = !grouped ? 8u : paged ? uint32_t(std::min(t.kp.page_size, kTile)) : uint32_t(kTile);
+  auto cache_map = [&](CUtensorMap* m, const void* p) {
+    if (grouped) {
+      const uint64_t dims[4] = {64, 8, kKB, kv_rows / 8}, strides[3] = {D, 64, 8 * D};
+      const uint32_t bx[4] = {64, 8, uint32_t(kKB), box / 8};
+      return make_map_bf16(m, p, 4, dims, strides, bx);
+    }
+    const uint64_t dims[3] = {64, kv_rows, kKB}, strides[2] = {D, 64};
+    const uint32_t bx[3] = {64, 8, uint32_t(kKB)};
+    return make_map_bf16(m, p, 3, dims, strides, bx);
   };
+  auto node_map = [&](CUtensorMap* m, const void* p) {
+    const uint64_t dims[4] = {64, rows, kKB, uint64_t(t.kv_heads)}, strides[3] = {uint64_t(t.kv_heads) * D, 64, D};
+    const uint32_t bx[4] = {64, 8, uint32_t(kKB), 1};
+    return make_map_bf16(m, p, 4, dims, strides, bx);
+  };
+  const uint64_t qdims[3] = {D, uint64_t(t.heads), rows}, qstrides[2] = {D, uint64_t(t.heads) * D};
+  const uint32_t qbox[3] = {64, uint32_t(group), uint32_t(tpt)};
   CUtensorMap qm, km, vm, knm, vnm;
-  if (!make_map_3d_bf16(&qm, t.q, D, uint64_t(t.heads), rows, uint32_t(group), uint32_t(tpt)) ||
-      !map(&km, t.k_cache, kv_rows, D, box) || !map(&vm, t.v_cache, kv_rows, D, box) ||
-      !map(&knm, t.k_new, rows, uint64_t(t.kv_heads) * D, kTile) ||
-      !map(&vnm, t.v_new, rows, uint64_t(t.kv_heads) * D, kTile))
+  if (!make_map_bf16(&qm, t.q, 3, qdims, qstrides, qbox) || !cache_map(&km, t.k_cache) || !cache_map(&vm, t.v_cache) ||
+      !node_map(&knm, t.k_new) || !node_map(&vnm, t.v_new))
     return SB_INTERNAL;
   Args a{t.base, t.count, t.mask, t.k_new, t.v_new, t.k_cache, t.v_cache, t.out, int(t.batch), int(t.tokens),
-         int(t.heads), int(t.kv_heads), int(t.max_len), group, tpt, int((t.tokens + 31) / 32), t.kp, int(kv_rows),
+         int(t.heads), int(t.kv_heads), int(t.max_len), group, tpt, int((t.tokens + 31) / 32), t.kp, int(kv_rows), int(box),
          static_cast<Meta*>(t.workspace), static_cast<uint8_t*>(t.workspace) + kMetaBytes, t.err};
   // A block per SM, fewer when there are not that many tiles even at full lengths.
   const int per_item = tpt * (Wide ? 2 : 1);
