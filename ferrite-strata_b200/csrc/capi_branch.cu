@@ -64,9 +64,7 @@ int32_t strata_b200_tree_attention_bf16(const uint16_t* q, const uint16_t* k_new
              KvPages{}, workspace, out, status};
   if (!make_pages(block_table, max_len, kv_heads, page_size, num_pages, &a.kp)) return SB_INVALID_ARGUMENT;
   if (!block_table && max_len > INT32_MAX / kv_heads / batch) return SB_INVALID_ARGUMENT;
-  if (!aligned(q, 16) || !aligned(k_new, 16) || !aligned(v_new, 16) || !aligned(k_cache, 16) ||
-      !aligned(v_cache, 16) || !aligned(out, 16) || !aligned(workspace, 16) || !aligned(base, 4) ||
-      !aligned(mask, 4) || (count && !aligned(count, 4)) || (status && !aligned(status, 4)))
+  if (!aligned(base, 4) || !aligned(mask, 4) || (count && !aligned(count, 4)) || (status && !aligned(status, 4)))
     return SB_INVALID_ARGUMENT;
   return launch_tree_attention(a, S(stream));
 }

@@ -1080,6 +1080,11 @@ bool tree_attention_supported(int64_t tokens, int64_t heads, int64_t kv_heads, i
 int launch_tree_attention(const TreeArgs& a, cudaStream_t st) {
   if (!tree_attention_supported(a.tokens, a.heads, a.kv_heads, a.head_dim)) return SB_INVALID_ARGUMENT;
   if (a.batch == 0) return SB_OK;
+  for (const void* p : {static_cast<const void*>(a.q), static_cast<const void*>(a.k_new),
+                        static_cast<const void*>(a.v_new), static_cast<const void*>(a.k_cache),
+                        static_cast<const void*>(a.v_cache), static_cast<const void*>(a.out),
+                        static_cast<const void*>(a.workspace)})
+    if (!p || (reinterpret_cast<uintptr_t>(p) & 15)) return SB_INVALID_ARGUMENT;  // TMA and 16-byte accesses
   if (wide(a.tokens, a.heads, a.kv_heads))
     return a.head_dim == 128 ? launch<128, true>(a, st) : launch<64, true>(a, st);
   return a.head_dim == 128 ? launch<128, false>(a, st) : launch<64, false>(a, st);

@@ -42,6 +42,8 @@ const PatternRule kRules[] = {
     {"fused::rope", true, true, true, false, false, false},
     {"fused::swiglu", true, true, true, false, false, false},
     {"fused::attention", true, true, true, false, false, false},
+    {"fused::tree_attention", true, false, true, false, false, false},
+    {"fused::beam_select", true, true, false, false, false, false},
     {"fused::embed", true, true, true, false, false, false},
     {"fused::argmax", true, false, false, true, false, false},
     {"fused::vocab_argmax", true, false, false, true, false, false},

@@ -489,7 +489,8 @@ struct Lowerer {
   bool lower_node(int ni) {
     const Node& n = g.nodes[ni];
     if (n.op == STRATA_OP_INPUT) return true;
-    if (n.outputs.size() != 1 && !(n.op == STRATA_OP_CUSTOM && n.pattern.rfind("fused::quantize_", 0) == 0))
+    if (n.outputs.size() != 1 && !(n.op == STRATA_OP_CUSTOM && (n.pattern.rfind("fused::quantize_", 0) == 0 ||
+                                                                n.pattern == "fused::beam_select")))
       return decline("every kernel here is single-output; node `" + n.name + "` has " +
                      std::to_string(n.outputs.size()));
     const uint32_t out = n.outputs.empty() ? kNone : n.outputs[0];
@@ -825,6 +826,97 @@ struct Lowerer {
         st.v.push_back(table);
         st.reads.push_back(table);
       }
+    } else if (p == "fused::tree_attention") {
+      // A tree of drafted tokens per sequence: q, k, v [batch * tokens, .], the
+      // caches (or page pools), base and count [batch], mask words [batch *
+      // tokens, ceil(tokens / 32)], and for page pools the block table.
+      const uint32_t q = in(n, 0), k = in(n, 1), v = in(n, 2), kc = in(n, 3), vc = in(n, 4), base = in(n, 5),
+                     count = in(n, 6), mask = in(n, 7);
+      for (uint32_t x : {q, k, v, kc, vc, out})
+        if (!is_bf16(V(x).dt)) return decline("tree attention runs in bf16");
+      for (uint32_t x : {base, count, mask})
+        if (!is_i32(V(x).dt)) return decline("tree attention takes I32 lengths, counts and mask words");
+      if (V(kc).dims.size() != 4 || V(kc).dims != V(vc).dims)
+        fail(STRATA_INVALID_ARGUMENT, "kv caches must be [batch, kv_heads, max_len, head_dim]");
+      const int64_t ps = n.attr_int("page_size", 0);
+      const int64_t B = V(base).elements(), KVH = V(kc).dims[1], D = V(kc).dims[3];
+      int64_t L = V(kc).dims[2], pps = 0, npages = 0;
+      uint32_t table = kNone;
+      if (ps != 0) {
+        if (n.inputs.size() < 9) fail(STRATA_INVALID_ARGUMENT, "paged tree attention needs a block table (input 8)");
+        table = in(n, 8);
+        if (!is_i32(V(table).dt) || V(table).dims.size() != 2 || V(table).dims[0] != B)
+          fail(STRATA_INVALID_ARGUMENT, "the block table must be I32 [batch, pages_per_seq]");
+        if (!sb::kv_page_size_ok(ps) || L != ps)
+          fail(STRATA_INVALID_ARGUMENT, "page_size must be a power of two from 16 to 4096 and the pages' length");
+        npages = V(kc).dims[0];
+        pps = V(table).dims[1];
+        L = pps * ps;
+        if (npages <= 0 || pps <= 0 || L > INT32_MAX || npages * KVH * ps > INT32_MAX)
+          fail(STRATA_INVALID_ARGUMENT, "paged tree attention pool or table is empty or too large");
+      } else if (V(kc).dims[0] != B || B * KVH * L > INT32_MAX) {
+        fail(STRATA_INVALID_ARGUMENT, "tree attention caches do not match the batch or are too large");
+      }
+      const int64_t H = n.attr_int("num_heads", 0), rows = rows_of(V(q));
+      if (n.attr_int("num_kv_heads", KVH) != KVH || n.attr_int("head_dim", D) != D)
+        fail(STRATA_INVALID_ARGUMENT, "attention attributes disagree with the cache shape");
+      if (H <= 0 || KVH <= 0 || H % KVH || B <= 0 || B > 65535 || rows % B || last_dim(V(q)) != H * D ||
+          last_dim(V(k)) != KVH * D || rows_of(V(k)) != rows || !same_dims(k, v) || !same_dims(q, out) ||
+          V(count).elements() != B)
+        fail(STRATA_INVALID_ARGUMENT, "tree attention operand shapes are inconsistent");
+      const int64_t T = rows / B;
+      if (V(mask).elements() != rows * ((T + 31) / 32))
+        fail(STRATA_INVALID_ARGUMENT, "tree attention needs ceil(tokens / 32) mask words per row");
+      if (!sb::tree_attention_supported(T, H, KVH, D))
+        return decline("tree attention: at most 1024 tokens, 128 query heads per kv head, head_dim 64 or 128");
+      st.kind = SK::TreeAttention;
+      st.bf16 = true;
+      st.i[0] = B;
+      st.i[1] = T;
+      st.i[2] = H;
+      st.i[3] = KVH;
+      st.i[4] = D;
+      st.i[5] = L;
+      st.i[7] = ps;
+      st.i[8] = pps;
+      st.i[9] = npages;
+      st.scratch_bytes = sb::tree_attention_workspace_bytes(T, H, KVH, D);
+      st.v = {q, k, v, kc, vc, base, count, mask, out};
+      st.reads = {q, k, v, kc, vc, base, count, mask};
+      st.writes = {out, kc, vc};
+      if (table != kNone) {
+        st.v.push_back(table);
+        st.reads.push_back(table);
+      }
+    } else if (p == "fused::beam_select") {
+      // logits [batch * beams, vocab], scores and done [batch * beams] ->
+      // scores, parent rows, tokens and done [batch * keep].
+      const uint32_t x = in(n, 0), sc = in(n, 1), dn = in(n, 2);
+      if (n.outputs.size() != 4) return decline("beam_select returns scores, parents, tokens and done");
+      if (!is_float(V(x).dt) || !is_f32(V(sc).dt) || !is_i32(V(dn).dt) || !is_f32(V(out).dt) ||
+          !is_i32(V(n.outputs[1]).dt) || !is_i32(V(n.outputs[2]).dt) || !is_i32(V(n.outputs[3]).dt))
+        return decline("beam_select maps f32/bf16 logits, F32 scores and I32 flags to F32 scores and I32 rows, ids, flags");
+      const int64_t rows = rows_of(V(x)), W = n.attr_int("beams", 0), keep = n.attr_int("keep", W),
+                    vocab = last_dim(V(x)), eos = n.attr_int("eos", -1);
+      if (W <= 0 || rows % W || V(sc).elements() != rows || V(dn).elements() != rows)
+        fail(STRATA_INVALID_ARGUMENT, "beam_select needs one score and one flag per row and whole sets of beams");
+      for (uint32_t o : n.outputs)
+        if (V(o).elements() != rows / W * keep)
+          fail(STRATA_INVALID_ARGUMENT, "beam_select outputs must have keep elements per sentence");
+      if (eos < -1 || eos >= vocab) fail(STRATA_INVALID_ARGUMENT, "beam_select eos is not a token id");
+      if (!sb::beam_select_supported(rows / W, W, vocab, keep))
+        return decline("beam_select: at most 1024 beams, 64 kept, 65535 rows, 2^30 tokens");
+      st.kind = SK::BeamSelect;
+      st.bf16 = is_bf16(V(x).dt);
+      st.i[0] = rows / W;
+      st.i[1] = W;
+      st.i[2] = vocab;
+      st.i[3] = keep;
+      st.i[4] = eos;
+      st.scratch_bytes = sb::beam_select_workspace_bytes(rows / W, W, vocab, keep);
+      st.v = {x, sc, dn, n.outputs[0], n.outputs[1], n.outputs[2], n.outputs[3]};
+      st.reads = {x, sc, dn};
+      st.writes = {n.outputs[0], n.outputs[1], n.outputs[2], n.outputs[3]};
     } else if (p == "fused::embed") {
       const uint32_t ids = in(n, 0), tab = in(n, 1);
       if (!is_i32(V(ids).dt) || !is_float(V(tab).dt) || !(V(out).dt == V(tab).dt) ||
@@ -1186,6 +1278,8 @@ const char* step_class(const Step& st) {
     case SK::QkvRope: return "gemv:qkv_rope_append";
     case SK::Attention: return "attention";
     case SK::KvAppend: return "kv_append";
+    case SK::TreeAttention: return "tree_attention";
+    case SK::BeamSelect: return "beam_select";
     case SK::AllReduce: return "all_reduce";
     case SK::AllReduceAddNorm: return "all_reduce_add_norm";
     case SK::RmsNorm: return "rms_norm";
@@ -1377,6 +1471,25 @@ void enqueue_steps(Ctx& ctx, Exe& exe, const std::vector<void*>& ext, StepEvents
             fail(STRATA_INTERNAL, std::string("ncclAllReduce failed: ") + ctx.nccl.error_string(r));
           rc = sb::launch_vocab_argmax_decode(keys, rows, out, s);
         }
+        break;
+      }
+      case SK::TreeAttention: {
+        const sb::TreeArgs a{P<uint16_t>(p, st.v[0]), P<uint16_t>(p, st.v[1]), P<uint16_t>(p, st.v[2]),
+                             P<uint16_t>(p, st.v[3]), P<uint16_t>(p, st.v[4]), P<int32_t>(p, st.v[5]),
+                             P<int32_t>(p, st.v[6]), P<uint32_t>(p, st.v[7]), st.i[0], st.i[1], st.i[2], st.i[3],
+                             st.i[4], st.i[5], pages_of(p, st, 9), static_cast<char*>(p.exe.ws) + st.scratch_off,
+                             P<uint16_t>(p, st.v[8]), ctx.d_err};
+        rc = sb::launch_tree_attention(a, s);
+        break;
+      }
+      case SK::BeamSelect: {
+        const auto run = [&](auto* x) {
+          return sb::launch_beam_select(x, P<float>(p, st.v[1]), P<int32_t>(p, st.v[2]), st.i[0], st.i[1], st.i[2],
+                                        st.i[3], st.i[4], P<float>(p, st.v[3]), P<int32_t>(p, st.v[4]),
+                                        P<int32_t>(p, st.v[5]), P<int32_t>(p, st.v[6]),
+                                        static_cast<char*>(p.exe.ws) + st.scratch_off, s);
+        };
+        rc = st.bf16 ? run(P<const uint16_t>(p, st.v[0])) : run(P<const float>(p, st.v[0]));
         break;
       }
       case SK::AllReduce: {

@@ -10,6 +10,7 @@
 #include <vector>
 
 #include "../../../include/strata_b200.h"
+#include "../k_branch.cuh"
 #include "../k_elem.cuh"
 #include "../k_gemv_mma.cuh"
 #include "wire.hpp"
@@ -74,7 +75,7 @@ struct Ctx {
 enum class SK {
   Linear, RmsNorm, Rope, SwiGLU, Binary, Unary, Softmax, LayerNorm, Transpose, Slice,
   Broadcast, Copy, Embed, Argmax, LastToken, GemmF32, KvAppend, Attention, AllReduce, AllReduceAddNorm,
-  Quant4, Quant8, Dequant4, Dequant8, QkvRope, VocabArgmax,
+  Quant4, Quant8, Dequant4, Dequant8, QkvRope, VocabArgmax, TreeAttention, BeamSelect,
 };
 
 struct Step {

@@ -22,6 +22,12 @@ fused::attention            q [R,H*d], k [R,G*d], v [R,G*d],           num_heads
                             k_cache, v_cache [B,G,L,d], pos I32 [R]    num_kv_heads, head_dim
                             paged: pools [P,G,ps,d], pos, then a       page_size (ps)
                             block table I32 [B, L/ps]
+fused::tree_attention       q [R,H*d], k [R,G*d], v [R,G*d], caches    num_heads,
+                            (or pools), base I32 [B], count I32 [B],   num_kv_heads, head_dim
+                            mask I32 [R, ceil(T/32)], paged: table     page_size (ps)
+fused::beam_select          logits [B*W,V], scores f32 [B*W],          beams (W), keep, eos
+                            done I32 [B*W] -> scores, parents,
+                            tokens, done, each [B*keep]
 fused::embed                ids I32 [R], table [V,D]
 fused::argmax               x [R,C] -> I32 [R] (lowest index on ties)
 fused::vocab_argmax         logits shard [R,Vr] -> I32 [R]: the argmax   vocab_offset (id of column 0)
@@ -33,6 +39,11 @@ fused::last_token           x [B*S,C] -> [B,C], each sequence's last row  tokens
 ``fused::attention`` appends row r's k/v at ``pos[r]`` of sequence
 ``r // (R / B)`` in the caches (an in-place update of two inputs) and then
 attends over positions ``0..pos[r]``; causality comes from the positions.
+``fused::tree_attention`` serves T drafted tokens per sequence: node t's k/v go to
+position ``base + t``, and it attends to the positions below ``base`` and to the
+live nodes (``t < count``) whose bit of its mask row is set.
+``fused::beam_select`` picks the ``keep`` best continuations of every sentence's
+W beams; ``parents`` are row ids.
 Tensor-parallel builds shard q/k/v/gate/up by output column and o/down by
 input row, with an all-reduce after o_proj and after down_proj only.  With
 the argmax head the lm_head is vocabulary-parallel: each rank holds the rows
@@ -86,6 +97,12 @@ class DecoderHandles:
     out: int = -1               # argmax ids, logits, or the last hidden state
     hidden_out: int = -1
     block_table: int = -1       # paged caches: I32 [batch, pages_per_seq], shared by every layer
+    base: int = -1              # tree steps: cached positions I32 [batch]
+    count: int = -1             # tree steps: live nodes I32 [batch]
+    mask: int = -1              # tree steps: mask words I32 [batch * tree, ceil(tree / 32)]
+    scores: int = -1            # beam head: accumulated log probabilities F32 [batch]
+    done: int = -1              # beam head: flags of ended beams I32 [batch]
+    beam_outs: tuple = ()       # beam head: scores, parents, tokens, done (``out`` is the tokens)
 
 
 def ffn_unit(fmt: str) -> int:
@@ -177,7 +194,7 @@ def decoder_graph(shape: DecoderShape, *, batch: int, seq: int, max_len: int, fm
                   layers: int | None = None, embed: bool = True, head: str = "argmax",
                   lm_fmt: str | None = None, tp_rank: int = 0, tp_world: int = 1,
                   last_token: bool = False, kv_page: int = 0, kv_pages: int | None = None,
-                  name: str = "decoder"):
+                  tree: bool = False, beams: int = 0, eos: int = -1, name: str = "decoder"):
     """One forward step of ``layers`` decoder blocks over ``batch * seq`` rows.
 
     ``seq == 1`` is a decode step; ``seq > 1`` a prefill from position 0 (the
@@ -190,7 +207,18 @@ def decoder_graph(shape: DecoderShape, *, batch: int, seq: int, max_len: int, fm
     ``I32 [batch, ceil(max_len / kv_page)]`` (``block_table``) maps every
     sequence's positions to pages; a sequence's capacity is then a whole
     number of pages.
+    ``tree`` makes the step a drafted tree of ``seq`` nodes per sequence: ``pos``
+    holds each node's position in its branch (base + depth, for RoPE), and
+    ``base``, ``count`` and ``mask`` say what is cached, which nodes are live and
+    what each node sees.  ``head="beam"`` ends a decode step in a beam selection:
+    the batch is whole sets of ``beams`` rows, each continued by its ``beams`` best
+    candidates; ``scores`` and ``done`` come in and, with the parents and tokens,
+    go out (``beam_outs``).
     """
+    if head == "beam" and (beams < 1 or batch % beams or tp_world > 1 or not (seq == 1 or last_token)):
+        raise ValueError("the beam head needs whole sets of beams, one row per beam, and no tensor parallelism")
+    if tree and (fmt == "f32" or last_token):
+        raise ValueError("a tree step runs in bf16 and keeps every node's row")
     layers = shape.layers if layers is None else layers
     act = F32 if fmt == "f32" else BF16
     D, H, G, d = shape.hidden, shape.heads, shape.kv_heads, shape.head_dim
@@ -210,6 +238,13 @@ def decoder_graph(shape: DecoderShape, *, batch: int, seq: int, max_len: int, fm
         npages = batch * pps if kv_pages is None else kv_pages
         hd.block_table = b.input(I32, (batch, pps), "block_table")
         attn_attrs = {"page_size": kv_page}
+    if tree:
+        hd.base = b.input(I32, (batch,), "tree_base")
+        hd.count = b.input(I32, (batch,), "tree_count")
+        hd.mask = b.input(I32, (R, -(-seq // 32)), "tree_mask")
+    if head == "beam":
+        hd.scores = b.input(F32, (batch,), "beam_scores")
+        hd.done = b.input(I32, (batch,), "beam_done")
     wshapes = weight_shapes(shape, fmt, t, tp_rank)
     for li in range(layers):
         W = {k: b.input(dt, dims, f"l{li}.{k}") for k, (dt, dims) in wshapes.items()}
@@ -256,8 +291,9 @@ def decoder_graph(shape: DecoderShape, *, batch: int, seq: int, max_len: int, fm
         rope_attrs = {"head_dim": d, "theta": float(shape.theta)}
         qr = b.node(Op.custom("fused::rope"), [q, hd.pos], [(act, (R, Hl * d))], rope_attrs, p + "q_rope")[0]
         kr = b.node(Op.custom("fused::rope"), [k, hd.pos], [(act, (R, Gl * d))], rope_attrs, p + "k_rope")[0]
-        ains = [qr, kr, v, W["k_cache"], W["v_cache"], hd.pos] + ([hd.block_table] if kv_page else [])
-        o = b.node(Op.custom("fused::attention"), ains, [(act, (R, Hl * d))],
+        where = [hd.base, hd.count, hd.mask] if tree else [hd.pos]
+        ains = [qr, kr, v, W["k_cache"], W["v_cache"], *where] + ([hd.block_table] if kv_page else [])
+        o = b.node(Op.custom("fused::tree_attention" if tree else "fused::attention"), ains, [(act, (R, Hl * d))],
                    {"num_heads": Hl, "num_kv_heads": Gl, "head_dim": d, **attn_attrs}, p + "attention")[0]
         a = _linear(b, o, W, "o", R, D, fmt, act, p + "o_proj")
         if t > 1:
@@ -287,12 +323,19 @@ def decoder_graph(shape: DecoderShape, *, batch: int, seq: int, max_len: int, fm
         logits = _linear(b, hf, W, "lm", Rh, Vr, lm_fmt or fmt, act, "lm_head")
         if head == "logits":
             hd.out = logits
+        elif head == "beam":
+            hd.beam_outs = tuple(b.node(
+                Op.custom("fused::beam_select"), [logits, hd.scores, hd.done],
+                [(F32, (Rh,)), (I32, (Rh,)), (I32, (Rh,)), (I32, (Rh,))],
+                {"beams": beams, "keep": beams, "eos": eos}, "beam_select"))
+            hd.out = hd.beam_outs[2]
         elif vpar:
             hd.out = b.node(Op.custom("fused::vocab_argmax"), [logits], [(I32, (Rh,))],
                             {"vocab_offset": v0}, "vocab_argmax")[0]
         else:
             hd.out = b.node(Op.custom("fused::argmax"), [logits], [(I32, (Rh,))], {}, "argmax")[0]
-    b.output(hd.out)
+    for o in hd.beam_outs or (hd.out,):
+        b.output(o)
     return b.build(), hd
 
 

@@ -43,6 +43,78 @@ def _threads() -> int:
     return ora.max_threads()
 
 
+def _tree_attention(ins, attrs):
+    """Node t of sequence b appends its k and v at base[b] + t and attends to the
+    positions below base[b] and to the live nodes whose mask bit it has; in f64,
+    position by position.  Caches (or page pools) are updated in place."""
+    q, kn, vn, kc, vc, base, count, mask = ins[:8]
+    H, G, d = int(attrs["num_heads"]), int(attrs["num_kv_heads"]), int(attrs["head_dim"])
+    ps = int(attrs.get("page_size", 0))
+    B = base.size
+    T = q.size // (H * d) // B
+    words = np.asarray(mask).view(np.uint32).reshape(B, T, -1)
+    q = q.reshape(B, T, H, d).astype(np.float64)
+    out = np.zeros((B, T, H, d))
+
+    def at(b, p):
+        return (int(ins[8][b, p // ps]), p % ps) if ps else (b, p)
+
+    for b in range(B):
+        n, p0 = int(count.reshape(-1)[b]), int(base.reshape(-1)[b])
+        for t in range(n):
+            f, r = at(b, p0 + t)
+            kc[f, :, r] = kn.reshape(B, T, G, d)[b, t]
+            vc[f, :, r] = vn.reshape(B, T, G, d)[b, t]
+        spots = [at(b, p) for p in range(p0 + n)]
+        if not spots:
+            continue
+        f, r = np.array(spots).T
+        K, V = kc[f, :, r].astype(np.float64), vc[f, :, r].astype(np.float64)  # [positions, G, d]
+        for t in range(n):
+            see = np.array([True] * p0 + [bool(words[b, t, j // 32] >> (j % 32) & 1) for j in range(n)])
+            if not see.any():
+                continue
+            for h in range(H):
+                s = K[see, h // (H // G)] @ q[b, t, h] / np.sqrt(d)
+                w = np.exp(s - s.max())
+                out[b, t, h] = w @ V[see, h // (H // G)] / w.sum()
+    return out.reshape(B * T, H * d).astype(np.float32)
+
+
+def _beam_select(logits, scores, done, attrs):
+    """The keep best (score + log-probability, lowest beam * vocab + token on
+    ties) of every sentence, in f64: scores, parent rows, tokens, done."""
+    W, eos = int(attrs["beams"]), int(attrs.get("eos", -1))
+    keep = int(attrs.get("keep", W))
+    x = np.asarray(logits, np.float64).reshape(-1, logits.shape[-1])
+    x = np.where(np.isnan(x), -np.inf, x)
+    R, V = x.shape
+    rows = [[], [], [], []]
+    for b in range(R // W):
+        cand = []
+        for r in range(b * W, (b + 1) * W):
+            s = float(np.asarray(scores).reshape(-1)[r])
+            if not s > -np.inf:
+                continue
+            if np.asarray(done).reshape(-1)[r]:
+                cand.append((-s, (r - b * W) * V + max(eos, 0), r, eos, 1))
+                continue
+            m = x[r].max()
+            if m == -np.inf:
+                continue
+            with np.errstate(invalid="ignore"):
+                y = np.where(x[r] == m, 0.0, x[r] - m)
+            y = y - np.log(np.exp(y).sum())
+            best = np.lexsort((np.arange(V), -y))[:keep]
+            cand += [(-(s + y[v]), (r - b * W) * V + v, r, int(v), int(v == eos)) for v in best if y[v] > -np.inf]
+        cand = sorted(cand)[:keep]
+        cand += [(np.inf, 0, -1, -1, 0)] * (keep - len(cand))
+        rows[0] += [-c[0] for c in cand]
+        for i in (1, 2, 3):
+            rows[i] += [c[i + 1] for c in cand]
+    return [np.array(rows[0], np.float32)] + [np.array(r, np.int32) for r in rows[1:]]
+
+
 def evaluate(graph, inputs: dict, all_reduce=None, all_gather=None) -> dict:
     """Run `graph` on the oracle.  `inputs` maps value id -> array; KV caches
     are updated in place in the returned dict.  `all_reduce(name, x)` sums
@@ -151,6 +223,13 @@ def evaluate(graph, inputs: dict, all_reduce=None, all_gather=None) -> dict:
                     kc[seq[r], :, p, :] = knr[r]
                     vc[seq[r], :, p, :] = vnr[r]
             res = ora.attention(q, kc, vc, seq, pos, H, G, d, threads=_threads())
+        elif pid == "fused::tree_attention":
+            res = _tree_attention(ins, n.attrs)
+        elif pid == "fused::beam_select":
+            outs = _beam_select(ins[0], ins[1], ins[2], n.attrs)
+            for o, r in zip(n.outputs, outs):
+                vals[o] = r.reshape(graph.values[o].dims)
+            continue
         elif pid == "fused::embed":
             res, _rc = ora.embed(ins[0], ins[1])
         elif pid == "fused::argmax":
