@@ -361,6 +361,28 @@ def test_tree_attention_empty_and_full_masks(cuda, lib):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("B,T,H,G,d,page,top,extra", [
+    (230, 4, 8, 4, 128, 0, 300, 3),    # several sequences a block, a cache of an odd length
+    (230, 9, 4, 2, 64, 16, 500, 0),
+    (60, 40, 16, 2, 128, 0, 700, 0),   # two query tiles of one kv head at once, the second often empty
+    (70, 33, 32, 4, 64, 16, 600, 0),
+    (3, 20, 16, 2, 128, 0, 9000, 5),   # one sequence over many blocks, many tiles each
+])
+def test_tree_attention_many_sequences_with_stale_rows(cuda, lib, B, T, H, G, d, page, top, extra):
+    """Blocks that go through several sequences, or through one for long, with
+    ragged counts and NaN in every row that no live position holds."""
+    rng = np.random.default_rng(B + T)
+    base, count = rng.integers(0, top, B), rng.integers(0, T + 1, B)
+    base[:3], count[:3] = [top, 0, top - 1], [T, 1, 1]
+    L = -(-(top + T + extra) // (page or 1)) * (page or 1)
+    if not page:
+        L += (extra - L) % 8  # a multiple of 8, or off by `extra`
+    t = Tree(B, B, T, H, G, d, L, base, count=count, page=page)
+    t.stale(np.nan)
+    t.go(cuda, lib)
+
+
+@pytest.mark.gpu
 def test_tree_attention_large_scores(cuda, lib):
     """Scores far apart: the running maximum moves by hundreds between tiles."""
     t = Tree(8, 2, 12, 4, 2, 128, 700, [600, 650])
