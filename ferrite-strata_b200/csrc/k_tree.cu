@@ -546,113 +546,127 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (si > 0) wait_bar(q_full, (si - 1) & 1);
     }
   } else if (warp == 1) {
-    // ---- products (lane 0 issues; the warp waits) ---------------------------------
+    // ---- products (one lane issues; the warp waits) ---------------------------------
+    // This warp shares its scheduler with the softmax, so what it does per product
+    // is kept short: descriptors differ by an addition, ring places by a step.
     constexpr uint32_t kIdS = idesc_bf16(kTile, kTile), kIdO = idesc_bf16(kTile, D, true);
-    int c0 = 0, si = 0;
-    int np[2] = {0, 0};  // P tiles of each group so far
+    constexpr uint32_t kSlotStep = L::kBytesTile >> 4;  // in descriptor units
+    const uint64_t q_desc = sw128_desc(smem + L::kQ), k_desc = sw128_desc(smem + L::kRing, L::kGroup),
+                   v_desc = sw128_desc_mn(smem + L::kRing, 1024, L::kGroup);
+    static_assert(kNS > 2, "a step of two loads passes the ring's end at most once");
+    struct Place {  // of a ring load
+      uint32_t slot, parity;
+      __device__ void step(uint32_t by) {
+        slot += by;
+        if (slot >= uint32_t(kNS)) {
+          slot -= kNS;
+          parity ^= 1;
+        }
+      }
+    };
+    Place first{0, 0};  // the segment's first load
+    int si = 0;
+    uint32_t np = 0;  // parity of each group's next P tile
     bool ok = true;
-    auto wait_load = [&](int c) { return wait_bar_warp(&full[c % kNS], (c / kNS) & 1); };
-    auto slot_of = [&](int c) { return smem + L::kRing + (c % kNS) * L::kBytesTile; };
-    auto release = [&](int c) {
-      if (lane == 0) umma_commit(&empty[c % kNS]);
-      __syncwarp();
+    auto wait_load = [&](const Place& c) { return wait_bar_warp(&full[c.slot], c.parity); };
+    auto release = [&](const Place& c) {
+      if (elect_one()) umma_commit(&empty[c.slot]);
     };
     auto release_q = [&]() {
-      if (lane == 0) umma_commit(q_empty);
-      __syncwarp();
+      if (elect_one()) umma_commit(q_empty);
     };
-    auto issue_s = [&](int t, const uint8_t* q, const uint8_t* k) {
+    auto wait_p = [&](int t) {
+      const bool r = wait_bar_warp(&p_full[t], np >> t & 1);
+      np ^= 1u << t;
+      return r;
+    };
+    auto issue_s = [&](int t, uint32_t tile, const Place& k) {
+      const uint64_t da = q_desc + uint64_t(tile * kSlotStep), db = k_desc + uint64_t(k.slot * kSlotStep);
       tc_fence_after();
-      if (lane == 0) {
+      if (elect_one()) {
 #pragma unroll
-        for (int kb = 0; kb < L::kKB; ++kb) {
-          const uint64_t da = sw128_desc(q + kb * 16384), db = sw128_desc(k + kb * 1024, L::kGroup);
+        for (int kb = 0; kb < L::kKB; ++kb)
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
-            umma_bf16(tmem + uint32_t(t * 128), da + uint64_t(2 * kk), db + uint64_t(2 * kk), kIdS, (kb | kk) != 0);
-        }
+            umma_bf16(tmem + uint32_t(t * 128), da + uint64_t(kb * (16384 >> 4) + 2 * kk),
+                      db + uint64_t(kb * (1024 >> 4) + 2 * kk), kIdS, (kb | kk) != 0);
         umma_commit(&s_full[t]);
       }
-      __syncwarp();
     };
-    const uint8_t* q0 = smem + L::kQ;
     for (;;) {
       if (!(ok = __all_sync(0xffffffffu, wait_seg(si)))) break;
       const Seg g = s_seg[si % kSegs];
       const int n = g.j1 - g.j0;
       if (n == 0) break;
       const bool second = Wide ? g.pair * per_item + a.tpt < g.s.count : n > 1;  // the second group has work
-      auto k_load = [&](int i) { return i == 0 ? c0 : c0 + 2 * i - 1; };
-      auto v_load = [&](int i) { return i == n - 1 ? c0 + 2 * n - 1 : c0 + 2 * i + 2; };
-      if (!(ok = wait_bar_warp(q_full, si & 1) && wait_load(k_load(0)))) break;
-      issue_s(0, q0, slot_of(k_load(0)));
-      if constexpr (Wide) {
-        if (second) issue_s(1, q0 + L::kBytesTile, slot_of(k_load(0)));
-        release(k_load(0));
-        if (n == 1) release_q();
-      } else {
-        release(k_load(0));
+      Place k = first, v = first;  // of the next K tile and the next V tile
+      v.step(n > 1 ? 2 : 1);
+      if (!(ok = wait_bar_warp(q_full, si & 1) && wait_load(k))) break;
+      issue_s(0, 0, k);
+      if (Wide && second) issue_s(1, 1, k);
+      release(k);
+      k.step(1);
+      if constexpr (!Wide) {
         if (second) {
-          if (!(ok = wait_load(k_load(1)))) break;
-          issue_s(1, q0, slot_of(k_load(1)));
-          release(k_load(1));
+          if (!(ok = wait_load(k))) break;
+          issue_s(1, 0, k);
+          release(k);
+          k.step(2);
         }
-        if (n <= 2) release_q();
       }
+      if (n == 1 || (!Wide && n == 2)) release_q();
       for (int i = 0; i < n && ok; ++i) {
-        uint8_t* v = slot_of(v_load(i));
-        if (!(ok = wait_load(v_load(i)))) break;
+        if (!(ok = wait_load(v))) break;
         int node0;
-        const int nv = tile_valid(g.s, g.j0 + i, node0), nv16 = (nv + 15) & ~15;
+        const int steps = (tile_valid(g.s, g.j0 + i, node0) + 15) / 16;
         // O of the segment before must have been read before this one's first P V.
         if (i == 0 && si >= 1 && !(ok = wait_bar_warp(o_free, (si - 1) & 1))) break;
-        const uint64_t vd = sw128_desc_mn(v, 1024, L::kGroup);
-        auto issue_o = [&](int t, bool first, bool last) {
+        const uint64_t dv = v_desc + uint64_t(v.slot * kSlotStep);
+        auto issue_o = [&](int t, bool first_pv, bool last_pv) {
+          const uint32_t tP = tmem + uint32_t(t * 128), tO = tmem + L::kOCol + uint32_t(t * D);
           tc_fence_after();
-          if (lane == 0) {
-            const uint32_t tP = tmem + uint32_t(t * 128), tO = tmem + L::kOCol + uint32_t(t * D);
+          if (elect_one()) {
+            umma_bf16_ts(tO, tP, dv, kIdO, !first_pv);
 #pragma unroll
-            for (int kk = 0; kk < kTile / 16; ++kk)
-              if (kk < nv16 / 16)
-                umma_bf16_ts(tO, tP + uint32_t(kk * 8), vd + uint64_t(kk * (2 * L::kGroup >> 4)), kIdO, !(first && kk == 0));
-            if (last) umma_commit(&o_done[t]);
+            for (int kk = 1; kk < kTile / 16; ++kk)
+              if (kk < steps) umma_bf16_ts(tO, tP + uint32_t(kk * 8), dv + uint64_t(kk * (2 * L::kGroup >> 4)), kIdO, 1);
+            if (last_pv) umma_commit(&o_done[t]);
           }
-          __syncwarp();
         };
+        const int ahead = Wide ? i + 1 : i + 2;  // the tile whose S follows this one's P V
         if constexpr (Wide) {
-          if (i + 1 < n && !(ok = wait_load(k_load(i + 1)))) break;
-          for (int t = 0; t < (second ? 2 : 1) && ok; ++t) {
-            if (!(ok = wait_bar_warp(&p_full[t], np[t] & 1))) break;
-            ++np[t];
+          if (ahead < n && !(ok = wait_load(k))) break;
+          for (int t = 0; t < (second ? 2 : 1); ++t) {
+            if (!(ok = wait_p(t))) break;
             issue_o(t, i == 0, i == n - 1);
-            if (i + 1 < n) issue_s(t, q0 + t * L::kBytesTile, slot_of(k_load(i + 1)));
+            if (ahead < n) issue_s(t, t, k);
           }
           if (!ok) break;
-          release(v_load(i));
-          if (i + 1 < n) release(k_load(i + 1));
-          if (i == n - 2) release_q();
+          release(v);
         } else {
           const int t = i & 1;
-          if (!(ok = wait_bar_warp(&p_full[t], np[t] & 1))) break;
-          ++np[t];
-          issue_o(t, i < 2, i + 2 >= n);
-          release(v_load(i));
-          if (i + 2 < n) {
-            if (!(ok = wait_load(k_load(i + 2)))) break;
-            issue_s(t, q0, slot_of(k_load(i + 2)));
-            release(k_load(i + 2));
-            if (i + 3 == n) release_q();
+          if (!(ok = wait_p(t))) break;
+          issue_o(t, i < 2, ahead >= n);
+          release(v);
+          if (ahead < n) {
+            if (!(ok = wait_load(k))) break;
+            issue_s(t, 0, k);
           }
         }
+        if (ahead < n) {
+          release(k);
+          k.step(2);
+          if (ahead == n - 1) release_q();
+        }
+        v.step(i + 2 >= n ? 1 : 2);  // the last V follows its K; past it the next segment starts
       }
       if (!ok) break;
-      c0 += 2 * n;
+      first = v;
       ++si;
       if (g.last) break;
     }
     if (!ok) fail();
-    if (lane == 0) umma_commit(mma_done);
-    __syncwarp();
+    if (elect_one()) umma_commit(mma_done);
     wait_bar_warp(mma_done, 0);
   } else if (warp == 2) {
     append_rows<D>(a, lane);
