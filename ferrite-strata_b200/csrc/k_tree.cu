@@ -87,11 +87,11 @@ struct Lay {
   static constexpr int kKB = D / 64;              // 64-wide blocks of head_dim
   static constexpr int kBytesTile = 128 * D * 2;  // a query tile: kKB blocks of [128 rows][128 bytes]
   static constexpr int kGroup = kKB * 1024;       // a K or V tile: 16 groups of kKB blocks of [8 rows][128 bytes]
-  static constexpr int kSlots = D == 128 ? 5 : 8;
+  static constexpr int kSlots = D == 128 ? (Wide ? 5 : 6) : (Wide ? 11 : 12);
   static constexpr int kQ = 0;
   static constexpr int kRing = (Wide ? 2 : 1) * kBytesTile;
-  static constexpr int kStat = kRing + kSlots * kBytesTile;  // sum [2 groups][2 halves][128], reference [2][128] (not wide)
-  static constexpr int kSeg = kStat + 4 * 128 * 4 + (Wide ? 0 : 2 * 128 * 4);
+  static constexpr int kStat = kRing + kSlots * kBytesTile;  // [2 groups][128]: sum and reference, or each half's sum (wide)
+  static constexpr int kSeg = kStat + 4 * 128 * 4;
   static constexpr int kBar = kSeg + kSegs * int(sizeof(Seg));
   static constexpr int kBars = 3 * kSlots + 12 + kSegs;
   static constexpr int kUse = kBar + kBars * 8 + 8 + 20;  // and the TMEM address, the failure word, four notes
@@ -107,7 +107,7 @@ struct Meta {
   int b, kvh, pair, count;
   int j0;  // the item's tile the run starts at (0: the run starts with the item)
   int nt;  // tiles of the item
-  int chunk, pad;
+  int share, extra;  // blocks below `extra` have share + 1 tiles, the others share
 };
 
 struct Args {
@@ -117,28 +117,32 @@ struct Args {
   uint16_t *k_cache, *v_cache, *out;
   int batch, tokens, heads, kv_heads, max_len;
   int group, tpt;  // query heads per kv head; nodes per query tile (tpt * group <= 128)
+  int per_item;    // nodes per item
+  uint32_t item_mul;  // ceil(2^20 / per_item)
   int words;       // mask words per node
   KvPages kp;
   int pool_rows;
+  int page_shift;  // log2 of the page size
   int box_rows;  // rows of a K or V box: 8, or a multiple of 8 that a map of whole groups gives
   Meta* meta;
   uint8_t* parts;
   int* err;
 };
 
-__device__ __forceinline__ Seq make_seq(const Args& a, int base, int count, int per_item, bool* bad = nullptr) {
-  Seq s{base, count, 0, 0, 0};
-  const bool wrong = s.count < 0 || s.count > a.tokens || s.base < 0 || s.base > a.max_len - s.count;
-  if (bad) *bad = wrong;
-  if (wrong) s.base = s.count = 0;
-  s.prefix = (s.base + kTile - 1) / kTile;
-  s.nt = s.count ? s.prefix + (s.count + kTile - 1) / kTile : 0;
-  s.pairs = (s.count + per_item - 1) / per_item;
-  return s;
+// Whether the call can serve the sequence; one that it cannot has nothing.
+__device__ __forceinline__ bool usable(const Args& a, int base, int count) {
+  return count >= 0 && count <= a.tokens && base >= 0 && base <= a.max_len - count;
 }
 
-__device__ __forceinline__ Seq seq_of(const Args& a, int b, int per_item, bool* bad = nullptr) {
-  return make_seq(a, a.base[b], a.count ? a.count[b] : a.tokens, per_item, bad);
+template <bool Wide>
+__device__ __forceinline__ Seq seq_of(const Args& a, int b) {
+  Seq s{a.base[b], a.count ? a.count[b] : a.tokens, 0, 0, 0};
+  if (!usable(a, s.base, s.count)) s.base = s.count = 0;
+  s.prefix = (s.base + kTile - 1) / kTile;
+  s.nt = s.count ? s.prefix + (s.count + kTile - 1) / kTile : 0;
+  // By multiplication: exact for what a tree can have (kTreeMaxTokens is below 2^11).
+  s.pairs = Wide ? int(uint32_t(s.count + a.per_item - 1) * a.item_mul >> 20) : s.count > 0;
+  return s;
 }
 
 // Where a block stands in its run.
@@ -148,22 +152,26 @@ struct Walk {
   uint32_t off;  // within sequence b's tiles
 };
 
-// The next segment; false at the run's end.  The host bounds all tiles of a
-// call below 2^31.
-__device__ __forceinline__ bool next_seg(const Args& a, int per_item, Walk& w, Seg& g) {
+// Tiles of a sequence.  The host bounds those of a call below 2^31.
+__device__ __forceinline__ uint32_t units_of(const Args& a, const Seq& s) {
+  return uint32_t(s.nt) * uint32_t(a.kv_heads) * uint32_t(s.pairs);
+}
+
+// The next segment; false at the run's end.
+template <bool Wide>
+__device__ __forceinline__ bool next_seg(const Args& a, Walk& w, Seg& g) {
   if (w.left <= 0) return false;
   for (;;) {
-    const uint32_t units = uint32_t(w.s.nt) * uint32_t(a.kv_heads) * uint32_t(w.s.pairs);
-    if (w.off < units) break;
+    if (w.off < units_of(a, w.s)) break;
     w.off = 0;  // runs end where sequences do
     if (++w.b >= a.batch) return false;
-    w.s = seq_of(a, w.b, per_item);
+    w.s = seq_of<Wide>(a, w.b);
   }
   g.s = w.s;
   g.b = w.b;
   const uint32_t item = w.off / uint32_t(w.s.nt);
   g.j0 = int(w.off - item * uint32_t(w.s.nt));
-  g.kvh = int(item / uint32_t(w.s.pairs));
+  g.kvh = int(Wide ? item / uint32_t(w.s.pairs) : item);
   g.pair = int(item - uint32_t(g.kvh) * uint32_t(w.s.pairs));
   g.j1 = min(w.s.nt, g.j0 + w.left);
   w.left -= g.j1 - g.j0;
@@ -188,9 +196,35 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity) {
   }
   return false;
 }
-// The same with one answer for the whole warp.
+// The same by a converged warp, whose lanes stay together.
 __device__ __forceinline__ bool wait_bar_warp(uint64_t* bar, uint32_t parity) {
-  return __all_sync(0xffffffffu, wait_bar(bar, parity));
+  const uint32_t at = su32(bar);
+#pragma unroll 1
+  for (uint32_t i = 0; i < kWaitLimit; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(done)
+        : "r"(at), "r"(parity)
+        : "memory");
+    if (__all_sync(0xffffffffu, done)) return true;
+  }
+  return false;
+}
+
+// An arrival by the lanes with `on`, without a branch: a warp that splits at
+// every arrival loses more than the arrival costs.
+__device__ __forceinline__ void arrive_if(bool on, uint64_t* bar) {
+  asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %1, 0;\n @p mbarrier.arrive.shared::cta.b64 _, [%0];\n}" ::"r"(su32(bar)),
+               "r"(uint32_t(on))
+               : "memory");
+}
+__device__ __forceinline__ void expect_if(bool on, uint64_t* bar, uint32_t bytes) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.u32 p, %2, 0;\n @p mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n}" ::"r"(
+          su32(bar)),
+      "r"(bytes), "r"(uint32_t(on))
+      : "memory");
 }
 
 // Tile j of a segment: valid positions, and for a tile of nodes the first node (-1 for cached positions).
@@ -262,10 +296,10 @@ __device__ void append_rows(const Args& a, int tid) {
 #pragma unroll 1
   for (int r = int(blockIdx.x); r < rows; r += int(gridDim.x)) {
     const int b = r / a.tokens, t = r % a.tokens;
-    bool bad;
-    const Seq s = seq_of(a, b, 1, &bad);
-    if (bad && t == 0 && tid == 0 && a.err) atomicExch(a.err, kBadPosition);
-    if (t >= s.count) {
+    const int base = a.base[b], count = a.count ? a.count[b] : a.tokens;
+    const bool good = usable(a, base, count);
+    if (!good && t == 0 && tid == 0 && a.err) atomicExch(a.err, kBadPosition);
+    if (!good || t >= count) {
       uint4* o = reinterpret_cast<uint4*>(a.out) + int64_t(r) * a.heads * kPer;
 #pragma unroll 1
       for (int i = tid; i < a.heads * kPer; i += kT) o[i] = make_uint4(0, 0, 0, 0);
@@ -273,7 +307,7 @@ __device__ void append_rows(const Args& a, int tid) {
     }
     const uint4* kn = reinterpret_cast<const uint4*>(a.k_new) + int64_t(r) * pieces;
     const uint4* vn = reinterpret_cast<const uint4*>(a.v_new) + int64_t(r) * pieces;
-    const int64_t row0 = kv_row(a.kp, b, 0, a.kv_heads, a.max_len, s.base + t);
+    const int64_t row0 = kv_row(a.kp, b, 0, a.kv_heads, a.max_len, base + t);
     if (row0 < 0) {
       if (tid == 0 && a.err) atomicExch(a.err, kBadPage);
       continue;
@@ -347,12 +381,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(words);
   int* s_fail = words + 1;
   int* s_odd = words + 2;  // [4]: s_odd[i % 4] == i + 1: segment i holds non-finite node values
-  float* s_sum = reinterpret_cast<float*>(smem + L::kStat);  // [group][half][row]
-  float* s_ref = s_sum + 4 * 128;                            // [group][row], not wide
+  float* s_stat = reinterpret_cast<float*>(smem + L::kStat);  // [group][2][row]
   Seg* s_seg = reinterpret_cast<Seg*>(smem + L::kSeg);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int per_item = a.tpt * (Wide ? 2 : 1);
+  const int per_item = a.per_item;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kNS; ++s) {
@@ -395,6 +428,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto fail = [&]() { atomicExch(s_fail, 1); };
   auto failed = [&]() { return *reinterpret_cast<volatile int*>(s_fail) != 0; };
 
+  static_assert(kNS > 2, "a step of two loads passes the ring's end at most once");
+  struct Place {  // of a ring load
+    uint32_t slot, parity;
+    __device__ void step(uint32_t by) {
+      slot += by;
+      if (slot >= uint32_t(kNS)) {
+        slot -= kNS;
+        parity ^= 1;
+      }
+    }
+  };
   // Every role takes the same segments from warp 0 and counts ring loads, S
   // tiles and segments for itself, so each barrier's phase is known without
   // any block-wide synchronisation.  Ring loads of a segment of n tiles that
@@ -406,127 +450,125 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 0) {
     // ---- the walk and the loads --------------------------------------------------
     // All tiles in one line, an equal run of it per block.
-    uint32_t total = 0, chunk = 0, w0 = 0;
+    uint32_t sum = 0, share = 0, extra = 0, w0 = 0, len = 0;
     Walk w{Seq{}, a.batch, 0, 0};
+    const int rounds = (a.batch + 31) / 32;
+    Seq s{};
 #pragma unroll 1
-    for (int pass = 0; pass < 2; ++pass) {  // the sum of all tiles; then where this block's run starts
-      uint32_t before = 0;
-#pragma unroll 1
-      for (int b0 = 0; b0 < a.batch; b0 += 32) {
-        int base = 0, count = 0;
-        if (b0 + lane < a.batch) {
-          base = a.base[b0 + lane];
-          count = a.count ? a.count[b0 + lane] : a.tokens;
-        }
-        const Seq s = make_seq(a, base, count, per_item);
-        const uint32_t u = uint32_t(s.nt) * uint32_t(a.kv_heads) * uint32_t(s.pairs);
-        uint32_t end = u;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const uint32_t y = __shfl_up_sync(0xffffffffu, end, o);
-          if (lane >= o) end += y;
-        }
-        end += before;
-        before = __shfl_sync(0xffffffffu, end, 31);
-        if (b0 + 32 >= a.batch && pass == 0) {
-          total = before;
-          chunk = (total + gridDim.x - 1) / gridDim.x;
-          w0 = chunk * blockIdx.x;
-        }
-        if ((pass == 1 || a.batch <= 32) && w0 < total) {
-          const uint32_t hit = __ballot_sync(0xffffffffu, w0 < end);
-          if (hit) {
-            const int l = __ffs(hit) - 1;
-            w.b = b0 + l;
-            w.off = w0 - (__shfl_sync(0xffffffffu, end, l) - __shfl_sync(0xffffffffu, u, l));
-            w.s = make_seq(a, __shfl_sync(0xffffffffu, base, l), __shfl_sync(0xffffffffu, count, l), per_item);
-            w.left = int(min(chunk, total - w0));
-            break;
-          }
-        }
+    for (int r = 0; r < 2 * rounds; ++r) {  // the sum of all tiles; then where this block's run starts
+      const int b0 = (r < rounds ? r : r - rounds) * 32;
+      if (r != 1 || rounds > 1) {  // one round of sequences is read once
+        s = Seq{};
+        if (b0 + lane < a.batch) s = seq_of<Wide>(a, b0 + lane);
       }
-      if (a.batch <= 32) break;
+      const uint32_t u = units_of(a, s);
+      if (r < rounds) {
+        sum += u;
+        if (r < rounds - 1) continue;
+        const uint32_t total = __reduce_add_sync(0xffffffffu, sum);
+        // A part costs about as much as a tile, so runs have two tiles at least
+        // (16 nodes over 500 positions, 32 heads: 15.6 -> 14.9 us).
+        const uint32_t blocks = min(gridDim.x, (total + 1) / 2);
+        share = blocks ? total / blocks : 0;
+        extra = total - share * blocks;
+        w0 = share * blockIdx.x + min(blockIdx.x, extra);
+        len = blockIdx.x < blocks ? share + (blockIdx.x < extra) : 0;
+        sum = 0;  // now of the sequences before
+        if (len == 0) break;
+        continue;
+      }
+      uint32_t end = u;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, end, o);
+        if (lane >= o) end += y;
+      }
+      end += sum;
+      const uint32_t hit = __ballot_sync(0xffffffffu, w0 < end);
+      if (hit) {
+        const int l = __ffs(hit) - 1;
+        w.b = b0 + l;
+        w.off = w0 - __shfl_sync(0xffffffffu, end - u, l);
+        w.s = Seq{__shfl_sync(0xffffffffu, s.base, l), __shfl_sync(0xffffffffu, s.count, l),
+                  __shfl_sync(0xffffffffu, s.prefix, l), __shfl_sync(0xffffffffu, s.nt, l),
+                  __shfl_sync(0xffffffffu, s.pairs, l)};
+        w.left = int(len);
+        break;
+      }
+      sum = __shfl_sync(0xffffffffu, end, 31);
     }
     int nl = 0, si = 0;
     bool ok = true;
+    Place next_load{0, 0};
     const int br = a.box_rows, nbox = kTile / br;
     Seg g;
-    Meta m{0, 0, 0, 0, 0, 0, int(chunk), 0};
+    Meta m{0, 0, 0, 0, 0, 0, int(share), int(extra)};
     if (w.left == 0 && lane == 0) {  // nothing to do: an empty segment ends every role
       s_seg[0] = Seg{Seq{}, 0, 0, 0, 0, 0, 1};
       mbar_arrive(&seg_full[0]);
     }
-    while (ok && next_seg(a, per_item, w, g)) {
+    while (ok && next_seg<Wide>(a, w, g)) {
       if (__any_sync(0xffffffffu, failed())) break;
+      if (!(ok = si == 0 || wait_bar_warp(q_empty, (si - 1) & 1))) break;
       if (lane == 0) {
-        if (si >= 1 && !wait_bar(q_empty, (si - 1) & 1)) ok = false;
-        if (ok) {
-          s_seg[si % kSegs] = g;
-          mbar_arrive(&seg_full[si % kSegs]);
-          const int t0 = g.pair * per_item;
-          const bool second = Wide && t0 + a.tpt < g.s.count;
-          const uint32_t bytes = uint32_t(L::kKB * a.tpt * a.group * 128);
-          mbar_expect_tx(q_full, second ? 2 * bytes : bytes);
-          for (int t = 0; t < (second ? 2 : 1); ++t)
-            for (int kb = 0; kb < L::kKB; ++kb)
-              tma_load_3d(smem + L::kQ + t * L::kBytesTile + kb * 16384, &qmap, q_full, kb * 64, g.kvh * a.group,
-                          g.b * a.tokens + t0 + t * a.tpt);
-        }
+        s_seg[si % kSegs] = g;
+        mbar_arrive(&seg_full[si % kSegs]);
       }
-      ok = __shfl_sync(0xffffffffu, ok, 0);
-      if (!ok) break;
+      const int t0 = g.pair * per_item;
+      const int qtiles = Wide && t0 + a.tpt < g.s.count ? 2 : 1;
+      if (lane == 0) mbar_expect_tx(q_full, uint32_t(qtiles * L::kKB * a.tpt * a.group * 128));
+      __syncwarp();
+      if (lane < qtiles * L::kKB) {
+        const int t = lane / L::kKB, kb = lane % L::kKB;
+        tma_load_3d(smem + L::kQ + t * L::kBytesTile + kb * 16384, &qmap, q_full, kb * 64, g.kvh * a.group,
+                    g.b * a.tokens + t0 + t * a.tpt);
+      }
       // This lane's box of tile j: the map row of its first position.  A page
       // that is missing is read past the map's end, which gives zeros.
       auto box_row = [&](int j) {
         if (j >= g.s.prefix || lane >= nbox) return 0;
         const int p = j * kTile + lane * br;
         if (!a.kp.paged()) return (g.b * a.kv_heads + g.kvh) * a.max_len + p;
-        const int64_t row = p < a.max_len ? kv_row(a.kp, g.b, g.kvh, a.kv_heads, a.max_len, p) : -1;
-        if (row < 0 && p < g.s.base && a.err) atomicExch(a.err, kBadPage);
-        return row < 0 ? a.pool_rows : int(row);
+        const int lp = p >> a.page_shift;
+        const int pg = lp < a.kp.pages_per_seq ? __ldg(a.kp.table + int64_t(g.b) * a.kp.pages_per_seq + lp) : -1;
+        if (uint32_t(pg) < uint32_t(a.kp.num_pages))
+          return ((pg * a.kv_heads + g.kvh) << a.page_shift) + (p & (a.kp.page_size - 1));
+        if (p < g.s.base && a.err) atomicExch(a.err, kBadPage);
+        return a.pool_rows;
       };
-      auto load = [&](int j, int row, bool is_v) {
-        const int slot = nl % kNS, round = nl / kNS;
+      auto load = [&](int tile, int map_row, bool is_v) {
+        uint64_t* bar = &full[next_load.slot];
+        uint8_t* dst = smem + L::kRing + next_load.slot * L::kBytesTile;
+        if (nl >= kNS && !wait_bar_warp(&empty[next_load.slot], next_load.parity ^ 1)) ok = false;
         int node0;
-        const int nv = tile_valid(g.s, j, node0);
-        uint64_t* bar = is_v && needs_cleaning(nv, node0) ? &raw[slot] : &full[slot];
-        if (lane == 0) {
-          if (round >= 1 && !wait_bar(&empty[slot], (round - 1) & 1)) ok = false;
-          // All of a cached tile; the 8-row groups of a tile of nodes that hold one.
-          if (ok) mbar_expect_tx(bar, j < g.s.prefix ? L::kBytesTile : (nv + 7) / 8 * L::kGroup);
-        }
-        ok = __shfl_sync(0xffffffffu, ok, 0);
+        const int nv = tile_valid(g.s, tile, node0);
+        if (is_v && needs_cleaning(nv, node0)) bar = &raw[next_load.slot];
         if (!ok) return;
-        uint8_t* dst = smem + L::kRing + slot * L::kBytesTile;
-        if (j < g.s.prefix) {
+        if (node0 < 0) {
+          expect_if(lane == 0, bar, L::kBytesTile);
           if (lane < nbox) {
-            uint8_t* at = dst + lane * (br / 8) * L::kGroup;
-            if (br > 8) tma_load_4d(at, is_v ? &vmap : &kmap, bar, 0, 0, 0, row / 8);
-            else tma_load_3d(at, is_v ? &vmap : &kmap, bar, 0, row, 0);
+            if (br > 8) tma_load_4d(dst + lane * (br / 8) * L::kGroup, is_v ? &vmap : &kmap, bar, 0, 0, 0, map_row / 8);
+            else tma_load_3d(dst + lane * L::kGroup, is_v ? &vmap : &kmap, bar, 0, map_row, 0);
           }
-        } else if (lane < (nv + 7) / 8) {
-          tma_load_4d(dst + lane * L::kGroup, is_v ? &vnmap : &knmap, bar, 0,
-                      g.b * a.tokens + (j - g.s.prefix) * kTile + lane * 8, 0, g.kvh);
+        } else {  // the 8-row groups that hold nodes
+          expect_if(lane == 0, bar, (nv + 7) / 8 * L::kGroup);
+          if (lane < (nv + 7) / 8)
+            tma_load_4d(dst + lane * L::kGroup, is_v ? &vnmap : &knmap, bar, 0, g.b * a.tokens + node0 + lane * 8, 0,
+                        g.kvh);
         }
+        next_load.step(1);
         ++nl;
       };
-      // K_0, then K_1, V_0, K_2, V_1, ..., and the last V: load i of the segment
-      // is the K tile (i + 1) / 2 for odd i (and i = 0), else the V tile i / 2 - 1.
-      // Map rows of the next V tile, the next K tile and the one after, so that the
-      // block table is read two tiles ahead.
-      const int n = g.j1 - g.j0;
-      int row = 0, next = box_row(g.j0), later = n > 1 ? box_row(g.j0 + 1) : 0;
+      // K_0, then K_1, V_0, K_2, V_1, ..., and the last V.  A tile's map rows are
+      // found two tiles before its K is loaded, so that the block table's latency is hidden.
+      int row = 0, next = 0, later = 0;  // of tiles j, j + 1, j + 2
 #pragma unroll 1
-      for (int i = 0; i < 2 * n && ok; ++i) {
-        const bool is_v = i == 2 * n - 1 || (i > 0 && !(i & 1));
-        const int j = g.j0 + (i == 2 * n - 1 ? n - 1 : is_v ? i / 2 - 1 : (i + 1) / 2);
-        load(j, is_v ? row : next, is_v);
-        if (is_v || i == 0) {  // the K tile loaded last is the next V tile
-          row = next;
-          next = later;
-          const int k = j + (is_v ? 3 : 2);
-          if (k < g.j1) later = box_row(k);
-        }
+      for (int j = g.j0 - 2; j < g.j1; ++j) {
+        row = next;
+        next = later;
+        if (j + 2 < g.j1) later = box_row(j + 2);
+        if (j >= g.j0 - 1 && j + 1 < g.j1) load(j + 1, next, false);
+        if (j >= g.j0) load(j, row, true);
       }
       if (si == 0) {
         m.b = g.b;
@@ -542,48 +584,31 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       a.meta[blockIdx.x] = m;
       // Let the loads in flight land before the block can end.
+#pragma unroll 1
       for (int c = max(0, nl - kNS); c < nl; ++c) wait_bar(&full[c % kNS], (c / kNS) & 1);
       if (si > 0) wait_bar(q_full, (si - 1) & 1);
     }
   } else if (warp == 1) {
-    // ---- products (one lane issues; the warp waits) ---------------------------------
-    // This warp shares its scheduler with the softmax, so what it does per product
-    // is kept short: descriptors differ by an addition, ring places by a step.
-    constexpr uint32_t kIdS = idesc_bf16(kTile, kTile), kIdO = idesc_bf16(kTile, D, true);
-    constexpr uint32_t kSlotStep = L::kBytesTile >> 4;  // in descriptor units
-    const uint64_t q_desc = sw128_desc(smem + L::kQ), k_desc = sw128_desc(smem + L::kRing, L::kGroup),
-                   v_desc = sw128_desc_mn(smem + L::kRing, 1024, L::kGroup);
-    static_assert(kNS > 2, "a step of two loads passes the ring's end at most once");
-    struct Place {  // of a ring load
-      uint32_t slot, parity;
-      __device__ void step(uint32_t by) {
-        slot += by;
-        if (slot >= uint32_t(kNS)) {
-          slot -= kNS;
-          parity ^= 1;
-        }
-      }
-    };
-    Place first{0, 0};  // the segment's first load
-    int si = 0;
-    uint32_t np = 0;  // parity of each group's next P tile
-    bool ok = true;
-    auto wait_load = [&](const Place& c) { return wait_bar_warp(&full[c.slot], c.parity); };
-    auto release = [&](const Place& c) {
-      if (elect_one()) umma_commit(&empty[c.slot]);
-    };
-    auto release_q = [&]() {
-      if (elect_one()) umma_commit(q_empty);
-    };
-    auto wait_p = [&](int t) {
-      const bool r = wait_bar_warp(&p_full[t], np >> t & 1);
-      np ^= 1u << t;
-      return r;
-    };
-    auto issue_s = [&](int t, uint32_t tile, const Place& k) {
-      const uint64_t da = q_desc + uint64_t(tile * kSlotStep), db = k_desc + uint64_t(k.slot * kSlotStep);
-      tc_fence_after();
-      if (elect_one()) {
+    // ---- products: one thread --------------------------------------------------------
+    // It shares its scheduler with the softmax, so what it does per product is
+    // kept short: no votes, descriptors differ by an addition, ring places by a step.
+    if (elect_one()) {
+      constexpr uint32_t kIdS = idesc_bf16(kTile, kTile), kIdO = idesc_bf16(kTile, D, true);
+      constexpr uint32_t kSlotStep = L::kBytesTile >> 4;  // in descriptor units
+      const uint64_t q_desc = sw128_desc(smem + L::kQ), k_desc = sw128_desc(smem + L::kRing, L::kGroup),
+                     v_desc = sw128_desc_mn(smem + L::kRing, 1024, L::kGroup);
+      Place first{0, 0};  // the segment's first load
+      int si = 0;
+      uint32_t np = 0;  // parity of each group's next P tile
+      bool ok = true;
+      auto wait_load = [&](const Place& c) { return wait_bar(&full[c.slot], c.parity); };
+      auto wait_p = [&](int t) {
+        const bool r = wait_bar(&p_full[t], np >> t & 1);
+        np ^= 1u << t;
+        return r;
+      };
+      auto issue_s = [&](int t, uint32_t tile, const Place& k) {
+        const uint64_t da = q_desc + uint64_t(tile * kSlotStep), db = k_desc + uint64_t(k.slot * kSlotStep);
 #pragma unroll
         for (int kb = 0; kb < L::kKB; ++kb)
 #pragma unroll
@@ -591,83 +616,82 @@ __global__ void __launch_bounds__(kThreads, 1)
             umma_bf16(tmem + uint32_t(t * 128), da + uint64_t(kb * (16384 >> 4) + 2 * kk),
                       db + uint64_t(kb * (1024 >> 4) + 2 * kk), kIdS, (kb | kk) != 0);
         umma_commit(&s_full[t]);
-      }
-    };
-    for (;;) {
-      if (!(ok = __all_sync(0xffffffffu, wait_seg(si)))) break;
-      const Seg g = s_seg[si % kSegs];
-      const int n = g.j1 - g.j0;
-      if (n == 0) break;
-      const bool second = Wide ? g.pair * per_item + a.tpt < g.s.count : n > 1;  // the second group has work
-      Place k = first, v = first;  // of the next K tile and the next V tile
-      v.step(n > 1 ? 2 : 1);
-      if (!(ok = wait_bar_warp(q_full, si & 1) && wait_load(k))) break;
-      issue_s(0, 0, k);
-      if (Wide && second) issue_s(1, 1, k);
-      release(k);
-      k.step(1);
-      if constexpr (!Wide) {
-        if (second) {
-          if (!(ok = wait_load(k))) break;
-          issue_s(1, 0, k);
-          release(k);
-          k.step(2);
+      };
+      for (;;) {
+        if (!(ok = wait_seg(si))) break;
+        const Seg g = s_seg[si % kSegs];
+        const int n = g.j1 - g.j0;
+        if (n == 0) break;
+        const bool second = Wide ? g.pair * per_item + a.tpt < g.s.count : n > 1;  // the second group has work
+        Place k = first, v = first;  // of the next K tile and the next V tile
+        v.step(n > 1 ? 2 : 1);
+        if (!(ok = wait_bar(q_full, si & 1) && wait_load(k))) break;
+        tc_fence_after();
+        issue_s(0, 0, k);
+        if (Wide && second) issue_s(1, 1, k);
+        umma_commit(&empty[k.slot]);
+        k.step(1);
+        if constexpr (!Wide) {
+          if (second) {
+            if (!(ok = wait_load(k))) break;
+            issue_s(1, 0, k);
+            umma_commit(&empty[k.slot]);
+            k.step(2);
+          }
         }
-      }
-      if (n == 1 || (!Wide && n == 2)) release_q();
-      for (int i = 0; i < n && ok; ++i) {
-        if (!(ok = wait_load(v))) break;
-        int node0;
-        const int steps = (tile_valid(g.s, g.j0 + i, node0) + 15) / 16;
+        if (n == 1 || (!Wide && n == 2)) umma_commit(q_empty);
         // O of the segment before must have been read before this one's first P V.
-        if (i == 0 && si >= 1 && !(ok = wait_bar_warp(o_free, (si - 1) & 1))) break;
-        const uint64_t dv = v_desc + uint64_t(v.slot * kSlotStep);
-        auto issue_o = [&](int t, bool first_pv, bool last_pv) {
-          const uint32_t tP = tmem + uint32_t(t * 128), tO = tmem + L::kOCol + uint32_t(t * D);
-          tc_fence_after();
-          if (elect_one()) {
+        if (si >= 1 && !(ok = wait_bar(o_free, (si - 1) & 1))) break;
+#pragma unroll 1
+        for (int i = 0; i < n; ++i) {
+          int node0;
+          const int steps = (tile_valid(g.s, g.j0 + i, node0) + 15) / 16;
+          const uint64_t dv = v_desc + uint64_t(v.slot * kSlotStep);
+          auto issue_o = [&](int t, bool first_pv, bool last_pv) {
+            const uint32_t tP = tmem + uint32_t(t * 128), tO = tmem + L::kOCol + uint32_t(t * D);
+            tc_fence_after();
             umma_bf16_ts(tO, tP, dv, kIdO, !first_pv);
 #pragma unroll
             for (int kk = 1; kk < kTile / 16; ++kk)
               if (kk < steps) umma_bf16_ts(tO, tP + uint32_t(kk * 8), dv + uint64_t(kk * (2 * L::kGroup >> 4)), kIdO, 1);
             if (last_pv) umma_commit(&o_done[t]);
-          }
-        };
-        const int ahead = Wide ? i + 1 : i + 2;  // the tile whose S follows this one's P V
-        if constexpr (Wide) {
-          if (ahead < n && !(ok = wait_load(k))) break;
-          for (int t = 0; t < (second ? 2 : 1); ++t) {
+          };
+          const int ahead = Wide ? i + 1 : i + 2;  // the tile whose S follows this one's P V
+          if (!(ok = wait_load(v) && (ahead >= n || wait_load(k)))) break;
+          if constexpr (Wide) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              if (t == 1 && !second) break;
+              if (!(ok = wait_p(t))) break;
+              issue_o(t, i == 0, i == n - 1);
+              if (ahead < n) issue_s(t, t, k);
+            }
+            if (!ok) break;
+            umma_commit(&empty[v.slot]);
+          } else {
+            const int t = i & 1;
             if (!(ok = wait_p(t))) break;
-            issue_o(t, i == 0, i == n - 1);
-            if (ahead < n) issue_s(t, t, k);
+            issue_o(t, i < 2, ahead >= n);
+            umma_commit(&empty[v.slot]);
+            if (ahead < n) issue_s(t, 0, k);
           }
-          if (!ok) break;
-          release(v);
-        } else {
-          const int t = i & 1;
-          if (!(ok = wait_p(t))) break;
-          issue_o(t, i < 2, ahead >= n);
-          release(v);
           if (ahead < n) {
-            if (!(ok = wait_load(k))) break;
-            issue_s(t, 0, k);
+            umma_commit(&empty[k.slot]);
+            k.step(2);
+            if (ahead == n - 1) umma_commit(q_empty);
           }
+          v.step(i + 2 >= n ? 1 : 2);  // the last V follows its K; past it the next segment starts
         }
-        if (ahead < n) {
-          release(k);
-          k.step(2);
-          if (ahead == n - 1) release_q();
-        }
-        v.step(i + 2 >= n ? 1 : 2);  // the last V follows its K; past it the next segment starts
+        if (!ok) break;
+        first = v;
+        ++si;
+        if (g.last) break;
       }
-      if (!ok) break;
-      first = v;
-      ++si;
-      if (g.last) break;
+      if (!ok) fail();
+      umma_commit(mma_done);
+      wait_bar(mma_done, 0);
     }
-    if (!ok) fail();
-    if (elect_one()) umma_commit(mma_done);
-    wait_bar_warp(mma_done, 0);
+    __syncwarp();
   } else if (warp == 2) {
     append_rows<D>(a, lane);
   } else if (warp == 3) {
@@ -735,7 +759,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     for (int si = 0;; ++si) {
       if (failed()) ok = false;
-      if (ok && !wait_seg(si)) ok = false;
+      if (ok && !wait_bar_warp(&seg_full[si % kSegs], (si / kSegs) & 1)) ok = false;
       ok = !pair_any(pair_bar, !ok);
       if (!ok) {  // the segments may not be there: all softmax warps leave here
         fail();
@@ -761,9 +785,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             seen[0] &= live && w < a.words ? a.mask[qrow * a.words + w] : 0u;
             seen[1] &= live && w + 1 < a.words ? a.mask[qrow * a.words + w + 1] : 0u;
           }
-          if (ok && !wait_bar(&s_full[t], ns & 1)) ok = false;
+          if (ok && !wait_bar_warp(&s_full[t], ns & 1)) ok = false;
           ++ns;
-          __syncwarp();  // the poll may have split the warp; tcgen05.ld needs it whole
           tc_fence_after();
           if (warp_live) {
             uint32_t r[kHalf];
@@ -836,22 +859,27 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[t]);
+          arrive_if(lane == 0, &p_full[t]);
         }
       }
       // ---- output ----------------------------------------------------------------------
       // The statistics of the segment before have been read by everyone.
-      if (si >= 1 && ok && !wait_bar(o_free, (si - 1) & 1)) ok = false;
-      s_sum[(t * 2 + half) * 128 + row] = l;
-      if (!Wide && half == 0) s_ref[t * 128 + row] = m_ref;
+      if (si >= 1 && ok && !wait_bar_warp(o_free, (si - 1) & 1)) ok = false;
+      s_stat[(t * 2 + half) * 128 + row] = l;
+      if (!Wide) {  // the other group wants the row's sum and its reference
+        pair_sync(pair_bar);
+        if (half == 0) s_stat[t * 256 + row] = l + s_stat[t * 256 + 128 + row];
+        pair_sync(pair_bar);
+        if (half == 1) s_stat[t * 256 + 128 + row] = m_ref;
+      }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&st_full[t]);
+      arrive_if(lane == 0, &st_full[t]);
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         if (Wide && x != t) continue;
-        if (ok && !wait_bar(&st_full[x], si & 1)) ok = false;
+        if (ok && !wait_bar_warp(&st_full[x], si & 1)) ok = false;
         if (Wide ? mine : x < n) {
-          if (ok && !wait_bar(&o_done[x], no[x] & 1)) ok = false;
+          if (ok && !wait_bar_warp(&o_done[x], no[x] & 1)) ok = false;
           ++no[x];
         }
       }
@@ -859,10 +887,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       if (mine && warp_live && __all_sync(0xffffffffu, ok)) {
         float w0 = 1.0f, w1 = 0.0f;  // weights of O_0 and O_1 (not wide: both belong to the row)
-        l = s_sum[(t * 2) * 128 + row] + s_sum[(t * 2 + 1) * 128 + row];
-        if (!Wide) {
-          const float m0 = s_ref[row], m1 = n > 1 ? s_ref[128 + row] : -INFINITY;
-          const float l0 = s_sum[row] + s_sum[128 + row], l1 = s_sum[256 + row] + s_sum[384 + row];
+        if (Wide) {
+          l = s_stat[t * 256 + row] + s_stat[t * 256 + 128 + row];
+        } else {
+          const float m0 = s_stat[128 + row], m1 = n > 1 ? s_stat[384 + row] : -INFINITY;
+          const float l0 = s_stat[row], l1 = s_stat[256 + row];
           m_ref = fmaxf(m0, m1);
           w1 = n > 1 ? 1.0f : 0.0f;
           if (m_ref != -INFINITY) {
@@ -873,11 +902,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const bool whole = g.j0 == 0 && g.j1 == g.s.nt;
         const bool odd = *reinterpret_cast<volatile int*>(&s_odd[si & 3]) == si + 1;
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // a row that sees nothing: O is 0
+        const float inv = l == 0.0f ? 0.0f : __fdividef(1.0f, l);  // a row that sees nothing: O is 0
         // A cut item: this part's place (0: the block's run starts in it).
-        const int64_t slot = (int64_t(blockIdx.x) * 2 + (si == 0 ? 0 : 1)) * (Wide ? 2 : 1) + (Wide ? t : 0);
-        float4* po = reinterpret_cast<float4*>(a.parts + slot * L::kPart);
-        float2* pm = reinterpret_cast<float2*>(a.parts + slot * L::kPart + size_t(D / 4) * 128 * 16);
+        const uint32_t slot = (blockIdx.x * 2 + (si == 0 ? 0 : 1)) * (Wide ? 2 : 1) + (Wide ? t : 0);
+        float4* po = reinterpret_cast<float4*>(a.parts + slot * uint32_t(L::kPart));
+        float2* pm = reinterpret_cast<float2*>(po + (D / 4) * 128);
         uint16_t* orow = a.out + (qrow * a.heads + g.kvh * a.group + head) * D;
         constexpr int kCols = Wide ? D / 2 : D / 4;  // this thread's columns
         const int col0 = (Wide ? half : t * 2 + half) * kCols;
@@ -929,7 +958,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // O and the statistics have been read.
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(o_free);
+      arrive_if(lane == 0, o_free);
       if (g.last) break;
     }
     if (!ok) fail();
@@ -956,10 +985,14 @@ __global__ void __launch_bounds__(128) tree_join_kernel(const Args a) {
   const int c = int(blockIdx.x), row = int(threadIdx.x);
   const int t = Wide ? int(blockIdx.y) / (D / 8) : 0, col = int(blockIdx.y) % (D / 8);
   const Meta m = a.meta[c];
-  if (m.j0 == 0 || m.j0 > m.chunk) return;
+  const int before = m.share + (c - 1 < m.extra);  // tiles of block c - 1
+  if (m.j0 == 0 || m.j0 > before) return;
   const int tok = m.pair * a.tpt * (Wide ? 2 : 1) + t * a.tpt + row / a.group;
   if (row / a.group >= a.tpt || tok >= m.count) return;
-  const int parts = 2 + (m.nt - m.j0 - 1) / m.chunk;  // block c - 1's, then c, c + 1, ...
+  // Block c - 1's part, then those of c, c + 1, ...: first the longer blocks, then the others.
+  const int rest = m.nt - m.j0, longer = max(0, m.extra - c), in_longer = longer * (m.share + 1);
+  const int parts = 1 + (rest <= in_longer ? (rest + m.share) / (m.share + 1)
+                                           : longer + (rest - in_longer + m.share - 1) / m.share);
   float best = -INFINITY, l = 0.0f, o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
   for (int k0 = 0; k0 < parts; k0 += kJoinParts) {
     float2 ml[kJoinParts];
@@ -970,7 +1003,7 @@ __global__ void __launch_bounds__(128) tree_join_kernel(const Args a) {
       ml[q] = make_float2(-INFINITY, 0.0f);
       x[q][0] = x[q][1] = make_float4(0, 0, 0, 0);
       if (k < parts) {
-        const int64_t slot = (int64_t(c - 1 + k) * 2 + (k == 0 && m.j0 < m.chunk ? 1 : 0)) * (Wide ? 2 : 1) + t;
+        const int64_t slot = (int64_t(c - 1 + k) * 2 + (k == 0 && m.j0 < before ? 1 : 0)) * (Wide ? 2 : 1) + t;
         const uint8_t* p = a.parts + slot * L::kPart;
         ml[q] = reinterpret_cast<const float2*>(p + size_t(D / 4) * 128 * 16)[row];
         x[q][0] = reinterpret_cast<const float4*>(p)[(col * 2) * 128 + row];
@@ -1000,7 +1033,7 @@ __global__ void __launch_bounds__(128) tree_join_kernel(const Args a) {
     }
     best = top;
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const float inv = l == 0.0f ? 0.0f : __fdividef(1.0f, l);
   uint16_t* orow = a.out + ((int64_t(m.b) * a.tokens + tok) * a.heads + m.kvh * a.group + row % a.group) * D + col * 8;
   *reinterpret_cast<uint4*>(orow) = make_uint4(pack_bf2(o[0] * inv, o[1] * inv), pack_bf2(o[2] * inv, o[3] * inv),
                                                pack_bf2(o[4] * inv, o[5] * inv), pack_bf2(o[6] * inv, o[7] * inv));
@@ -1017,7 +1050,7 @@ int launch(const TreeArgs& t, cudaStream_t st) {
                                     L::kBytes) == cudaSuccess;
       }))
     return SB_INTERNAL;
-  const int group = int(t.heads / t.kv_heads), tpt = kTile / group;
+  const int group = int(t.heads / t.kv_heads), tpt = kTile / group, per_item = tpt * (Wide ? 2 : 1);
   const bool paged = t.kp.paged();
   const uint64_t rows = uint64_t(t.batch) * uint64_t(t.tokens);
   const uint64_t kv_rows = paged ? uint64_t(t.kp.num_pages) * uint64_t(t.kv_heads) * uint64_t(t.kp.page_size)
@@ -1053,10 +1086,9 @@ int launch(const TreeArgs& t, cudaStream_t st) {
       !node_map(&knm, t.k_new) || !node_map(&vnm, t.v_new))
     return SB_INTERNAL;
   Args a{t.base, t.count, t.mask, t.k_new, t.v_new, t.k_cache, t.v_cache, t.out, int(t.batch), int(t.tokens),
-         int(t.heads), int(t.kv_heads), int(t.max_len), group, tpt, int((t.tokens + 31) / 32), t.kp, int(kv_rows), int(box),
+         int(t.heads), int(t.kv_heads), int(t.max_len), group, tpt, per_item, ((1u << 20) + unsigned(per_item) - 1) / unsigned(per_item), int((t.tokens + 31) / 32), t.kp, int(kv_rows), paged ? __builtin_ctz(unsigned(t.kp.page_size)) : 0, int(box),
          static_cast<Meta*>(t.workspace), static_cast<uint8_t*>(t.workspace) + kMetaBytes, t.err};
   // A block per SM, fewer when there are not that many tiles even at full lengths.
-  const int per_item = tpt * (Wide ? 2 : 1);
   const int64_t tiles = (t.max_len + kTile - 1) / kTile + (t.tokens + kTile - 1) / kTile;
   const int64_t items = t.batch * t.kv_heads * ((t.tokens + per_item - 1) / per_item);
   if (items > INT32_MAX / tiles) return SB_INVALID_ARGUMENT;
