@@ -102,16 +102,18 @@ __global__ void __launch_bounds__(kCpThreads)
   pdl_trigger();
   pdl_wait();
   const int lane = threadIdx.x & 31;
-  const int pieces = (page_size * chunks + kPiece - 1) / kPiece;
-  const int64_t per = int64_t(n_pools) * kv_heads * pieces;
-  const int64_t units = per * *n_list;
-  const int64_t warps = int64_t(gridDim.x) * (kCpThreads / 32);
-  for (int64_t u = int64_t(blockIdx.x) * (kCpThreads / 32) + (threadIdx.x >> 5); u < units; u += warps) {
-    const PageCopy cp = list[u / per];
-    int64_t r = u % per;
-    const int piece = int(r % pieces);
-    r /= pieces;
-    const int h = int(r % kv_heads), pool = int(r / kv_heads);
+  const uint32_t pieces = uint32_t(page_size * chunks + kPiece - 1) / kPiece;
+  const uint32_t per = uint32_t(n_pools) * uint32_t(kv_heads) * pieces;  // below 2^31 (launcher)
+  const uint32_t warps = gridDim.x * (kCpThreads / 32), first = blockIdx.x * (kCpThreads / 32) + (threadIdx.x >> 5);
+  // (copy, unit within it), carried along instead of divided out: with all copies
+  // together a unit's number may pass 32 bits.
+  uint32_t copy = first / per, in = first - copy * per;
+  const uint32_t step_copy = warps / per, step_in = warps - step_copy * per;
+  const uint32_t copies = uint32_t(*n_list);
+  for (; copy < copies; copy += step_copy, in += step_in, copy += in >= per, in -= in >= per ? per : 0) {
+    const PageCopy cp = list[copy];
+    const uint32_t hp = in / pieces;
+    const int piece = int(in - hp * pieces), pool = int(hp / uint32_t(kv_heads)), h = int(hp) - pool * kv_heads;
     const int end = cp.rows * chunks, c0 = piece * kPiece;
     if (c0 >= end) continue;
     uint4* p = static_cast<uint4*>(pools.p[pool]);
@@ -133,24 +135,40 @@ __global__ void __launch_bounds__(kCpThreads)
 // ---------------------------------------------------------------------------
 constexpr int kPlThreads = 1024;
 constexpr int kPlMaxCluster = 8;
+constexpr int kPlItems = 4 * kPlThreads;  // table entries and pages that one block plans alone
+
+// Division of numbers below 2^31 by a fixed positive one: floor(n m / 2^(31 + s))
+// with m = ceil(2^(31 + s) / d) and 2^s >= d (Granlund and Montgomery 1994).
+struct FastDiv {
+  uint32_t m = 0;
+  int s = 0, d = 1;
+  FastDiv() = default;
+  explicit FastDiv(int div) : d(div) {
+    while ((int64_t(1) << s) < div) ++s;
+    m = uint32_t(((uint64_t(1) << (31 + s)) + unsigned(div) - 1) / unsigned(div));
+  }
+  __device__ __forceinline__ int div(int n) const { return int(uint64_t(uint32_t(n)) * m >> (31 + s)); }
+};
 
 // Exclusive prefix sum over the block's threads; *total gets the sum.
-__device__ __forceinline__ int block_scan(int v, int* warp_sums, int* total) {
+template <typename T>
+__device__ __forceinline__ T block_scan(T v, T* warp_sums, T* total) {
+  static_assert(kPlThreads == 1024, "one warp adds up the warps' sums");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int x = v;
-#pragma unroll
+  T x = v;
+#pragma unroll 1
   for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    const T y = __shfl_up_sync(0xffffffffu, x, o);
     if (lane >= o) x += y;
   }
   __syncthreads();
   if (lane == 31) warp_sums[warp] = x;
   __syncthreads();
   if (warp == 0) {
-    int s = lane < kPlThreads / 32 ? warp_sums[lane] : 0;
-#pragma unroll
+    T s = warp_sums[lane];
+#pragma unroll 1
     for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, s, o);
+      const T y = __shfl_up_sync(0xffffffffu, s, o);
       if (lane >= o) s += y;
     }
     warp_sums[lane] = s;
@@ -163,8 +181,9 @@ __device__ __forceinline__ int block_scan(int v, int* warp_sums, int* total) {
 struct ForkArgs {
   const int32_t *table_in, *lens_in, *refs_in, *parents;
   int32_t *table_out, *lens_out, *refs_out, *report;
-  int rows, per, page_size, num_pages, reserve;
-  // workspace
+  int rows, per, page_shift, num_pages, reserve;
+  FastDiv by_per;
+  // workspace; the first four in shared memory where one block plans
   int *left, *cand, *free_list, *row_off;
   PageCopy* copies;
   int* n_copies;
@@ -187,15 +206,16 @@ __device__ __forceinline__ ForkRow fork_row(const ForkArgs& a, int r) {
   }
   if (f.parent < 0) return f;
   f.len = a.lens_in[f.parent];
-  if (f.len < 0 || int64_t(f.len) + a.reserve > int64_t(a.per) * a.page_size) {
+  const int most = a.per << a.page_shift;  // below 2^31
+  if (f.len < 0 || f.len > most || a.reserve > most - f.len) {
     f.bad = true;
     f.len = 0;
     f.parent = -1;
     return f;
   }
-  f.full = f.len / a.page_size;
-  f.part = f.len % a.page_size;
-  f.need = (f.len + a.reserve + a.page_size - 1) / a.page_size;
+  f.full = f.len >> a.page_shift;
+  f.part = f.len - (f.full << a.page_shift);
+  f.need = int((uint32_t(f.len + a.reserve) + (1u << a.page_shift) - 1) >> a.page_shift);
   return f;
 }
 
@@ -207,33 +227,44 @@ __device__ __forceinline__ ForkRow fork_row(const ForkArgs& a, int r) {
 // or wants it; the free pages are dealt out in ascending order to the rows in
 // ascending order.  When something is wrong or the pool is short, the outputs
 // are the inputs and nothing is copied.
-__global__ void __launch_bounds__(kPlThreads) kv_fork_plan_kernel(const ForkArgs a) {
+__global__ void __launch_bounds__(kPlThreads) kv_fork_plan_kernel(const __grid_constant__ ForkArgs args) {
+  extern __shared__ int s_plan[];
   cg::cluster_group cluster = cg::this_cluster();
   const int nranks = int(cluster.num_blocks()), rank = int(cluster.block_rank());
   const int tid = rank * kPlThreads + threadIdx.x, nthreads = nranks * kPlThreads;
-  __shared__ int s_warp[32], s_err, s_low, s_free;
+  __shared__ long long s_warp[32];
+  __shared__ int s_err, s_low, s_free;
+  ForkArgs a = args;
+  if (nranks == 1) {
+    a.left = s_plan;
+    a.cand = a.left + a.num_pages;
+    a.free_list = a.cand + a.num_pages;
+    a.row_off = a.free_list + a.num_pages;
+  }
   if (threadIdx.x == 0) {
     s_err = 0;
     s_low = 0;
   }
   pdl_trigger();
   pdl_wait();
+#pragma unroll 1
   for (int g = tid; g < a.num_pages; g += nthreads) {
     a.left[g] = a.refs_in[g];
     a.cand[g] = kNobody;
   }
   cluster.sync();
   int err = 0;
-  const int64_t entries = int64_t(a.rows) * a.per;
-  for (int64_t e = tid; e < entries; e += nthreads) {
-    const int r = int(e / a.per), i = int(e % a.per);
+  const int entries = a.rows * a.per;
+#pragma unroll 1
+  for (int e = tid; e < entries; e += nthreads) {
+    const int r = a.by_per.div(e), i = e - r * a.per;
     const int old = a.table_in[e];
     if (old >= a.num_pages) err = max(err, kBadPage);
     const ForkRow f = fork_row(a, r);
     if (f.bad) err = max(err, kBadPosition);
     int mine = -1;
     if (f.parent >= 0 && (i < f.full || (i == f.full && f.part))) {
-      mine = f.parent == r ? old : a.table_in[int64_t(f.parent) * a.per + i];
+      mine = f.parent == r ? old : a.table_in[f.parent * a.per + i];
       if (mine < 0 || mine >= a.num_pages) {
         err = max(err, kBadPage);
         mine = -1;
@@ -249,10 +280,12 @@ __global__ void __launch_bounds__(kPlThreads) kv_fork_plan_kernel(const ForkArgs
   if (err) atomicMax(&s_err, err);
   cluster.sync();
   err = 0;
+#pragma unroll 1
   for (int k = 0; k < nranks; ++k) err = max(err, *cluster.map_shared_rank(&s_err, k));
   // Pages each row takes from the free list, and which rows copy: every block
   // scans all rows for itself, block 0 writes the offsets down.
   int total = 0, copies = 0;
+#pragma unroll 1
   for (int r0 = 0; r0 < a.rows; r0 += kPlThreads) {
     const int r = r0 + threadIdx.x;
     int take = 0, copy = 0, tail = -1;
@@ -262,18 +295,19 @@ __global__ void __launch_bounds__(kPlThreads) kv_fork_plan_kernel(const ForkArgs
       if (f.parent >= 0) {
         bool keep = false;
         if (f.part) {
-          tail = a.table_in[int64_t(f.parent) * a.per + f.full];
+          tail = a.table_in[f.parent * a.per + f.full];
           keep = a.left[tail] == 0 && a.cand[tail] == r;
           copy = !keep;
         }
         take = f.need - f.full - (keep ? 1 : 0);
       }
     }
-    int sum, nc;
-    const int off = total + block_scan(take, s_warp, &sum);
-    const int at = copies + block_scan(copy, s_warp, &nc);
-    total += sum;
-    copies += nc;
+    // Both sums in one scan: a block's rows copy at most 1024 pages.
+    long long sum;
+    const long long both = block_scan(static_cast<long long>(take) << 16 | copy, s_warp, &sum);
+    const int off = total + int(both >> 16), at = copies + int(both & 0xffff);
+    total += int(sum >> 16);
+    copies += int(sum & 0xffff);
     if (rank == 0 && r < a.rows) {
       a.row_off[r] = off;
       if (copy) a.copies[at] = PageCopy{tail, -1, f.part, r};
@@ -286,17 +320,19 @@ __global__ void __launch_bounds__(kPlThreads) kv_fork_plan_kernel(const ForkArgs
   const int g1 = min(g0 + run, min(a.num_pages, (rank + 1) * slice));
   int mine = 0;
   bool low = false;
+#pragma unroll 1
   for (int g = g0; g < g1; ++g) {
     const int l = a.left[g];
     mine += l == 0 && a.cand[g] == kNobody;
     low |= l < 0;
   }
-  int sum;
-  const int before = block_scan(mine, s_warp, &sum);
-  if (threadIdx.x == 0) s_free = sum;
+  long long sum;
+  const int before = int(block_scan(static_cast<long long>(mine), s_warp, &sum));
+  if (threadIdx.x == 0) s_free = int(sum);
   if (low) s_low = kBadRefs;
   cluster.sync();
   int free_pages = 0, ahead = 0;
+#pragma unroll 1
   for (int k = 0; k < nranks; ++k) {
     err = max(err, *cluster.map_shared_rank(&s_low, k));
     const int f = *cluster.map_shared_rank(&s_free, k);
@@ -305,6 +341,7 @@ __global__ void __launch_bounds__(kPlThreads) kv_fork_plan_kernel(const ForkArgs
   }
   if (!err && total > free_pages) err = kNoPages;
   int nth = ahead + before;
+#pragma unroll 1
   for (int g = g0; g < g1; ++g) {
     int refs = a.refs_in[g];
     if (!err) {
@@ -324,17 +361,18 @@ __global__ void __launch_bounds__(kPlThreads) kv_fork_plan_kernel(const ForkArgs
     a.refs_out[g] = refs;
   }
   cluster.sync();
-  for (int64_t e = tid; e < entries; e += nthreads) {
-    const int r = int(e / a.per), i = int(e % a.per);
+#pragma unroll 1
+  for (int e = tid; e < entries; e += nthreads) {
+    const int r = a.by_per.div(e), i = e - r * a.per;
     int v = a.table_in[e];
     if (!err) {
       const ForkRow f = fork_row(a, r);
-      const int got = f.parent >= 0 ? a.table_in[int64_t(f.parent) * a.per + i] : -1;
+      const int got = f.parent >= 0 ? a.table_in[f.parent * a.per + i] : -1;
       v = -1;
       if (f.parent >= 0 && i < f.need) {
         bool keep = false;
         if (f.part) {
-          const int tail = i == f.full ? got : a.table_in[int64_t(f.parent) * a.per + f.full];
+          const int tail = i == f.full ? got : a.table_in[f.parent * a.per + f.full];
           keep = a.left[tail] == 0 && a.cand[tail] == r;
         }
         if (i < f.full || (keep && i == f.full)) v = got;
@@ -343,8 +381,10 @@ __global__ void __launch_bounds__(kPlThreads) kv_fork_plan_kernel(const ForkArgs
     }
     a.table_out[e] = v;
   }
+#pragma unroll 1
   for (int r = tid; r < a.rows; r += nthreads) a.lens_out[r] = err ? a.lens_in[r] : fork_row(a, r).len;
   if (!err)
+#pragma unroll 1
     for (int k = tid; k < copies; k += nthreads) a.copies[k].dst = a.free_list[a.row_off[a.copies[k].pad]];
   if (tid == 0) {
     *a.n_copies = err ? 0 : copies;
@@ -386,6 +426,7 @@ __global__ void __launch_bounds__(kPlThreads) kv_compact_plan_kernel(const Compa
   const int g1 = min(g0 + run, min(a.num_pages, (rank + 1) * slice));
   int mine = 0;
   bool bad = false;
+#pragma unroll 1
   for (int g = g0; g < g1; ++g) {
     const int c = a.refs_in[g];
     mine += c > 0;
@@ -395,14 +436,16 @@ __global__ void __launch_bounds__(kPlThreads) kv_compact_plan_kernel(const Compa
   int before = block_scan(mine, s_warp, &sum);
   if (threadIdx.x == 0) s_used = sum;
   if (bad) atomicMax(&s_err, kBadRefs);
-  const int64_t entries = int64_t(a.rows) * a.per;
-  for (int64_t e = tid; e < entries; e += nthreads) {
+  const int entries = a.rows * a.per;
+#pragma unroll 1
+  for (int e = tid; e < entries; e += nthreads) {
     const int g = a.table_in[e];
     if (g >= a.num_pages) atomicMax(&s_err, kBadPage);
     else if (g >= 0 && a.refs_in[g] <= 0) atomicMax(&s_err, kBadRefs);
   }
   cluster.sync();
   int n = 0, err = 0;
+#pragma unroll 1
   for (int k = 0; k < nranks; ++k) {
     const int u = *cluster.map_shared_rank(&s_used, k);
     n += u;
@@ -412,6 +455,7 @@ __global__ void __launch_bounds__(kPlThreads) kv_compact_plan_kernel(const Compa
   // used(before n), found by the thread whose run holds page n (none does
   // when every page is used: then nothing moves).
   int used = before;
+#pragma unroll 1
   for (int g = g0; g < g1; ++g) {
     const bool u = a.refs_in[g] > 0;
     if (g == n) s_low = used;
@@ -420,10 +464,12 @@ __global__ void __launch_bounds__(kPlThreads) kv_compact_plan_kernel(const Compa
   }
   cluster.sync();
   int low = 0;
+#pragma unroll 1
   for (int k = 0; k < nranks; ++k) low += *cluster.map_shared_rank(&s_low, k);
   if (n == a.num_pages) low = n;
   const int moves = err ? 0 : n - low;
   used = before;
+#pragma unroll 1
   for (int g = g0; g < g1; ++g) {
     const int c = a.refs_in[g];
     const bool u = c > 0;
@@ -445,7 +491,8 @@ __global__ void __launch_bounds__(kPlThreads) kv_compact_plan_kernel(const Compa
     used += u;
   }
   cluster.sync();
-  for (int64_t e = tid; e < entries; e += nthreads) {
+#pragma unroll 1
+  for (int e = tid; e < entries; e += nthreads) {
     const int g = a.table_in[e];
     a.table_out[e] = err ? g : g < 0 ? -1 : a.remap[g];
   }
@@ -460,14 +507,15 @@ __global__ void __launch_bounds__(kPlThreads) kv_compact_plan_kernel(const Compa
 }
 
 template <typename Args>
-int launch_plan(void (*kern)(Args), const Args& a, int64_t items, cudaStream_t st) {
-  // One block up to 4096 items (table entries and pages): its barriers cost a
-  // tenth of a cluster's.  Then as many blocks as give each that many.
+int launch_plan(void (*kern)(Args), const Args& a, int64_t items, size_t shared, cudaStream_t st) {
+  // One block up to kPlItems: its barriers cost a tenth of a cluster's, and what it
+  // notes per page lies in shared memory.  Then as many blocks as give each that many.
   int blocks = 1;
-  while (blocks < kPlMaxCluster && int64_t(blocks) * 4 * kPlThreads < items) blocks *= 2;
+  while (blocks < kPlMaxCluster && int64_t(blocks) * kPlItems < items) blocks *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(blocks));
   cfg.blockDim = dim3(kPlThreads);
+  cfg.dynamicSmemBytes = blocks == 1 ? shared : 0;
   cfg.stream = st;
   cudaLaunchAttribute attrs[2];
   attrs[0].id = cudaLaunchAttributeClusterDimension;
@@ -483,11 +531,15 @@ int launch_plan(void (*kern)(Args), const Args& a, int64_t items, cudaStream_t s
   return SB_OK;
 }
 
+// What warps share out of one copied page; the copying kernel counts it in 31 bits.
+int64_t units_per_copy(int64_t n_pools, int64_t row_bytes, int64_t kv_heads, int64_t page_size) {
+  return n_pools * kv_heads * ((page_size * (row_bytes / 16) + kPiece - 1) / kPiece);
+}
+
 int launch_copies(const KvPools& pools, int64_t n_pools, int64_t row_bytes, int64_t kv_heads, int64_t page_size,
                   int64_t most, const PageCopy* list, const int* n_list, cudaStream_t st) {
   const int chunks = int(row_bytes / 16);
-  const int64_t pieces = (page_size * chunks + kPiece - 1) / kPiece;
-  const int64_t units = most * n_pools * kv_heads * pieces;
+  const int64_t units = most * units_per_copy(n_pools, row_bytes, kv_heads, page_size);
   const int64_t blocks = std::min<int64_t>((units + kCpThreads / 32 - 1) / (kCpThreads / 32), int64_t(kNumSMs) * 8);
   if (launch_pdl(page_copy_kernel, dim3(unsigned(std::max<int64_t>(blocks, 1))), dim3(kCpThreads), 0, st, pools,
                  int(n_pools), int(kv_heads), int(page_size), chunks, list, n_list) != cudaSuccess)
@@ -537,8 +589,10 @@ int launch_kv_fork(const KvPools& pools, int64_t n_pools, int64_t row_bytes, int
                    int64_t num_pages, const int32_t* table_in, const int32_t* lens_in, const int32_t* refs_in,
                    const int32_t* parents, int64_t rows, int64_t pages_per_seq, int64_t reserve, int32_t* table_out,
                    int32_t* lens_out, int32_t* refs_out, int32_t* report, void* workspace, cudaStream_t st) {
+  if (units_per_copy(n_pools, row_bytes, kv_heads, page_size) > INT32_MAX) return SB_INVALID_ARGUMENT;
   ForkArgs a{table_in, lens_in, refs_in, parents, table_out, lens_out, refs_out, report, int(rows),
-             int(pages_per_seq), int(page_size), int(num_pages), int(reserve), nullptr, nullptr, nullptr, nullptr,
+             int(pages_per_seq), __builtin_ctz(unsigned(page_size)), int(num_pages), int(reserve),
+             FastDiv(int(pages_per_seq)), nullptr, nullptr, nullptr, nullptr,
              nullptr, nullptr};
   Carve w{static_cast<uint8_t*>(workspace)};
   a.left = w.take<int>(uint64_t(num_pages));
@@ -547,7 +601,15 @@ int launch_kv_fork(const KvPools& pools, int64_t n_pools, int64_t row_bytes, int
   a.row_off = w.take<int>(uint64_t(rows));
   a.copies = w.take<PageCopy>(uint64_t(rows));
   a.n_copies = w.take<int>(1);
-  const int rc = launch_plan(kv_fork_plan_kernel, a, rows * pages_per_seq + num_pages, st);
+  // The pages and rows of a call that one block plans are at most kPlItems together.
+  static PerDeviceOnce configured;
+  if (!configured.run([] {
+        return cudaFuncSetAttribute(kv_fork_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    3 * kPlItems * 4) == cudaSuccess;
+      }))
+    return SB_INTERNAL;
+  const int rc = launch_plan(kv_fork_plan_kernel, a, rows * pages_per_seq + num_pages,
+                             size_t(3 * num_pages + rows) * 4, st);
   if (rc || n_pools == 0) return rc;
   return launch_copies(pools, n_pools, row_bytes, kv_heads, page_size, rows, a.copies, a.n_copies, st);
 }
@@ -560,13 +622,14 @@ int launch_kv_compact(const KvPools& pools, int64_t n_pools, int64_t row_bytes, 
                       int64_t num_pages, const int32_t* table_in, const int32_t* refs_in, int64_t rows,
                       int64_t pages_per_seq, int32_t* table_out, int32_t* refs_out, int32_t* remap, int32_t* report,
                       void* workspace, cudaStream_t st) {
+  if (units_per_copy(n_pools, row_bytes, kv_heads, page_size) > INT32_MAX) return SB_INVALID_ARGUMENT;
   CompactArgs a{table_in, refs_in, table_out, refs_out, remap, report, int(rows), int(pages_per_seq),
                 int(page_size), int(num_pages), nullptr, nullptr, nullptr};
   Carve w{static_cast<uint8_t*>(workspace)};
   a.holes = w.take<int>(uint64_t(num_pages));
   a.copies = w.take<PageCopy>(uint64_t(num_pages));
   a.n_copies = w.take<int>(1);
-  const int rc = launch_plan(kv_compact_plan_kernel, a, rows * pages_per_seq + num_pages, st);
+  const int rc = launch_plan(kv_compact_plan_kernel, a, rows * pages_per_seq + num_pages, 0, st);
   if (rc || n_pools == 0) return rc;
   return launch_copies(pools, n_pools, row_bytes, kv_heads, page_size, num_pages / 2 + 1, a.copies, a.n_copies, st);
 }
