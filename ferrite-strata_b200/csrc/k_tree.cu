@@ -61,6 +61,7 @@ using namespace tc;
 constexpr int kTile = 128;   // query rows per tile, positions per KV tile
 constexpr int kHalf = 64;    // positions per softmax thread
 constexpr int kThreads = 640;
+constexpr int kStart = 2;    // what starting an item costs, in tiles (see the walk)
 constexpr int kSegs = 4;     // segments the walking warp is ahead at most, rounded up
 constexpr uint32_t kTmemCols = 512;  // S_0, S_1 (128 columns each), O_0, O_1 (head_dim each)
 constexpr float kLog2e = 1.4426950408889634f;
@@ -107,7 +108,7 @@ struct Meta {
   int b, kvh, pair, count;
   int j0;  // the item's tile the run starts at (0: the run starts with the item)
   int nt;  // tiles of the item
-  int share, extra;  // blocks below `extra` have share + 1 tiles, the others share
+  int share, extra;  // blocks below `extra` have share + 1 units, the others share
 };
 
 struct Args {
@@ -145,19 +146,21 @@ __device__ __forceinline__ Seq seq_of(const Args& a, int b) {
   return s;
 }
 
-// Where a block stands in its run.
+// The line that blocks share out is counted in units: an item is kStart units
+// that stand for starting it and then its tiles, one unit each.
 struct Walk {
   Seq s;  // of sequence b
-  int b, left;
-  uint32_t off;  // within sequence b's tiles
+  int b, left;   // units left of the block's run
+  uint32_t off;  // within sequence b's units
 };
 
-// Tiles of a sequence.  The host bounds those of a call below 2^31.
+// Units of a sequence.  The host bounds those of a call below 2^31.
 __device__ __forceinline__ uint32_t units_of(const Args& a, const Seq& s) {
-  return uint32_t(s.nt) * uint32_t(a.kv_heads) * uint32_t(s.pairs);
+  return s.nt ? uint32_t(s.nt + kStart) * uint32_t(a.kv_heads) * uint32_t(s.pairs) : 0;
 }
 
-// The next segment; false at the run's end.
+// The next segment; false at the run's end.  A run holds a tile whenever `left`
+// is not 0: what remains of it is dropped when only start units do.
 template <bool Wide>
 __device__ __forceinline__ bool next_seg(const Args& a, Walk& w, Seg& g) {
   if (w.left <= 0) return false;
@@ -169,14 +172,16 @@ __device__ __forceinline__ bool next_seg(const Args& a, Walk& w, Seg& g) {
   }
   g.s = w.s;
   g.b = w.b;
-  const uint32_t item = w.off / uint32_t(w.s.nt);
-  g.j0 = int(w.off - item * uint32_t(w.s.nt));
+  const uint32_t per = uint32_t(w.s.nt + kStart), item = w.off / per;
+  const int at = int(w.off - item * per), units = min(int(per) - at, w.left);
+  g.j0 = max(0, at - kStart);
   g.kvh = int(Wide ? item / uint32_t(w.s.pairs) : item);
   g.pair = int(item - uint32_t(g.kvh) * uint32_t(w.s.pairs));
-  g.j1 = min(w.s.nt, g.j0 + w.left);
-  w.left -= g.j1 - g.j0;
-  w.off += uint32_t(g.j1 - g.j0);
-  g.last = w.left <= 0;
+  g.j1 = at + units - kStart;
+  w.off += uint32_t(units);
+  w.left -= units;
+  if (w.left <= kStart) w.left = 0;
+  g.last = w.left == 0;
   return true;
 }
 
@@ -449,7 +454,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto wait_seg = [&](int si) { return wait_bar(&seg_full[si % kSegs], (si / kSegs) & 1); };
   if (warp == 0) {
     // ---- the walk and the loads --------------------------------------------------
-    // All tiles in one line, an equal run of it per block.
+    // All items in one line, an equal run of it per block.  A block that goes on to
+    // another item drains its products, writes O and fills up again meanwhile: blocks
+    // with three segments finished 4 to 8 us behind those with two.  So a start counts
+    // as kStart tiles: 16 nodes over 500 positions, 32 heads, 14.5 -> 12.4 us (3: 12.6,
+    // 5: 13.8); 8 x 25 nodes over 1100 to 2048, 55.9 -> 53.7 us.
     uint32_t sum = 0, share = 0, extra = 0, w0 = 0, len = 0;
     Walk w{Seq{}, a.batch, 0, 0};
     const int rounds = (a.batch + 31) / 32;
@@ -466,7 +475,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         sum += u;
         if (r < rounds - 1) continue;
         const uint32_t total = __reduce_add_sync(0xffffffffu, sum);
-        // A part costs about as much as a tile, so runs have two tiles at least
+        // A part costs about as much as a tile, so runs have two units at least
         // (16 nodes over 500 positions, 32 heads: 15.6 -> 14.9 us).
         const uint32_t blocks = min(gridDim.x, (total + 1) / 2);
         share = blocks ? total / blocks : 0;
@@ -493,6 +502,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                   __shfl_sync(0xffffffffu, s.prefix, l), __shfl_sync(0xffffffffu, s.nt, l),
                   __shfl_sync(0xffffffffu, s.pairs, l)};
         w.left = int(len);
+        const uint32_t at = w.off % uint32_t(w.s.nt + kStart);
+        if (at + len <= kStart) w.left = 0;  // the next block has the item's first tile
         break;
       }
       sum = __shfl_sync(0xffffffffu, end, 31);
@@ -985,7 +996,7 @@ __global__ void __launch_bounds__(128) tree_join_kernel(const Args a) {
   const int c = int(blockIdx.x), row = int(threadIdx.x);
   const int t = Wide ? int(blockIdx.y) / (D / 8) : 0, col = int(blockIdx.y) % (D / 8);
   const Meta m = a.meta[c];
-  const int before = m.share + (c - 1 < m.extra);  // tiles of block c - 1
+  const int before = m.share + (c - 1 < m.extra);  // units of block c - 1
   if (m.j0 == 0 || m.j0 > before) return;
   const int tok = m.pair * a.tpt * (Wide ? 2 : 1) + t * a.tpt + row / a.group;
   if (row / a.group >= a.tpt || tok >= m.count) return;
@@ -1003,7 +1014,7 @@ __global__ void __launch_bounds__(128) tree_join_kernel(const Args a) {
       ml[q] = make_float2(-INFINITY, 0.0f);
       x[q][0] = x[q][1] = make_float4(0, 0, 0, 0);
       if (k < parts) {
-        const int64_t slot = (int64_t(c - 1 + k) * 2 + (k == 0 && m.j0 < before ? 1 : 0)) * (Wide ? 2 : 1) + t;
+        const int64_t slot = (int64_t(c - 1 + k) * 2 + (k == 0 && m.j0 + kStart < before ? 1 : 0)) * (Wide ? 2 : 1) + t;
         const uint8_t* p = a.parts + slot * L::kPart;
         ml[q] = reinterpret_cast<const float2*>(p + size_t(D / 4) * 128 * 16)[row];
         x[q][0] = reinterpret_cast<const float4*>(p)[(col * 2) * 128 + row];
@@ -1089,7 +1100,7 @@ int launch(const TreeArgs& t, cudaStream_t st) {
          int(t.heads), int(t.kv_heads), int(t.max_len), group, tpt, per_item, ((1u << 20) + unsigned(per_item) - 1) / unsigned(per_item), int((t.tokens + 31) / 32), t.kp, int(kv_rows), paged ? __builtin_ctz(unsigned(t.kp.page_size)) : 0, int(box),
          static_cast<Meta*>(t.workspace), static_cast<uint8_t*>(t.workspace) + kMetaBytes, t.err};
   // A block per SM, fewer when there are not that many tiles even at full lengths.
-  const int64_t tiles = (t.max_len + kTile - 1) / kTile + (t.tokens + kTile - 1) / kTile;
+  const int64_t tiles = (t.max_len + kTile - 1) / kTile + (t.tokens + kTile - 1) / kTile + kStart;  // and start units
   const int64_t items = t.batch * t.kv_heads * ((t.tokens + per_item - 1) / per_item);
   if (items > INT32_MAX / tiles) return SB_INVALID_ARGUMENT;
   const int64_t most = items * tiles;
