@@ -6,7 +6,12 @@
 //
 // All three move whole 16-byte pieces and compute nothing on them, so they
 // are exact in any element type; what bounds them is HBM (every moved byte is
-// read once and written once) or, for a few rows, latency.
+// read once and written once) or, for a few rows, latency.  Measured, device time
+// back to back in a graph: accepting one sequence's path in 64 caches 3.1 us (the
+// host's launch takes 9), 32 paths of up to 33 nodes in 160 pools 14.7 us; forking 4
+// rows of 64 pools 9.9 us, most of it the plan's chain of dependent reads; 128 rows of
+// 32 pools 46 us, the copies alone (220 MB) 39 us with nothing cached, 5.6 TB/s;
+// compacting 3000 pages of 32 pools 240 us, the copies 236 us, 6.1 TB/s.
 #include <cooperative_groups.h>
 
 #include <algorithm>
