@@ -470,19 +470,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     // 5: 13.8); 8 x 25 nodes over 1100 to 2048, 55.9 -> 53.7 us.
     uint32_t sum = 0, share = 0, extra = 0, w0 = 0, len = 0;
     Walk w{Seq{}, a.batch, 0, 0};
-    const int rounds = (a.batch + 31) / 32;
+    const int sets = (a.batch + 31) / 32;
     Seq s{};
 #pragma unroll 1
-    for (int r = 0; r < 2 * rounds; ++r) {  // the sum of all tiles; then where this block's run starts
-      const int b0 = (r < rounds ? r : r - rounds) * 32;
-      if (r != 1 || rounds > 1) {  // one round of sequences is read once
+    for (int r = 0; r < 2 * sets; ++r) {  // the sum of all tiles; then where this block's run starts
+      const int b0 = (r < sets ? r : r - sets) * 32;
+      if (r != 1 || sets > 1) {  // a single set of sequences is read once
         s = Seq{};
         if (b0 + lane < a.batch) s = seq_of<Wide>(a, b0 + lane);
       }
       const uint32_t u = units_of(a, s);
-      if (r < rounds) {
+      if (r < sets) {
         sum += u;
-        if (r < rounds - 1) continue;
+        if (r < sets - 1) continue;
         const uint32_t total = __reduce_add_sync(0xffffffffu, sum);
         // A part costs about as much as a tile, so runs have two units at least
         // (16 nodes over 500 positions, 32 heads: 15.6 -> 14.9 us).

@@ -88,6 +88,7 @@ class PagedKv:
             self._ptrs = (_P * pools)(*[b.device_ptr() for b in self.pools])
             self.side = 0
             self.lens = np.zeros(rows, np.int32)  # the host's copy of the rows' lengths
+            self.held = np.zeros(rows, np.int64)  # positions that each row has pages for
             self._table[0].write(np.full((rows, pages_per_row), -1, np.int32))
             self._refs[0].write(np.zeros(pages, np.int32))
         except Exception:
@@ -135,6 +136,8 @@ class PagedKv:
         report = self._check(rc, "kv_fork")
         self.side = b
         self.lens = np.where(parents >= 0, self.lens[np.maximum(parents, 0)], 0).astype(np.int32)
+        pages = -(-(self.lens.astype(np.int64) + reserve) // self.page_size)
+        self.held = np.where(parents >= 0, pages * self.page_size, 0)
         return report
 
     def compact(self) -> np.ndarray:
@@ -150,7 +153,8 @@ class PagedKv:
 
     def accept(self, paths) -> None:
         """Keeps, of each row's drafted rows from its length on, those of ``paths[r]`` (strictly
-        increasing node numbers) and moves the length past them."""
+        increasing node numbers, within the positions the row has pages for) and moves the length
+        past them."""
         width = max([len(p) for p in paths] + [1])
         if len(paths) != self.rows or width > 1024:
             raise ValueError("one path per row, of at most 1024 nodes")
@@ -158,6 +162,8 @@ class PagedKv:
         for r, p in enumerate(paths):
             if any(y <= x for x, y in zip([-1, *p], p)):
                 raise ValueError("a path is strictly increasing from 0 on")
+            if len(p) and self.lens[r] + p[-1] >= self.held[r]:
+                raise ValueError("a path ends past the row's pages")
             path[r, :len(p)] = p
         self._path.write(path)
         self._n.write(n)
@@ -298,7 +304,8 @@ class BeamDecoder(_Decoder):
         d.write(np.zeros(kv.rows, np.int32))
 
     def step(self):
-        """One step of every beam: (scores, parent rows, tokens, done), each [sentences, beams]."""
+        """One step of every beam: (scores, parent rows, tokens, done), each [sentences, beams].
+        After an error the search has to start again."""
         kv = self.kv
         self._pos.write(kv.lens)
         self._runs[kv.side, self._cur].run()

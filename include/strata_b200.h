@@ -199,7 +199,7 @@ int32_t strata_b200_argmax_bf16(const uint16_t *x, int64_t rows, int64_t cols,
  *    block_table is null, else page pools [num_pages, kv_heads, page_size,
  *    head_dim] with a block table I32 [batch, max_len / page_size] (page_size a
  *    power of two from 16 to 4096); batch (or pool) * kv_heads * positions is
- *    below 2^31.
+ *    below 2^31.  No two caches, pools or outputs of a call overlap.
  *  - A workspace is device memory of at least the bytes its *_workspace_bytes
  *    function gives (0 for a shape the entry point refuses), 16-byte aligned,
  *    whose contents do not matter before or after a call.  Two calls that may
@@ -223,7 +223,9 @@ int32_t strata_b200_argmax_bf16(const uint16_t *x, int64_t rows, int64_t cols,
  * base + count > max_len gets status 2: zeros, and nothing is appended.
  * Positions on missing pages get status 6 and read as zero rows.  tokens <=
  * 1024, head_dim 64 or 128, at most 128 query heads per kv head, pointers
- * 16-byte aligned.  Two sequences must not append to the same page. */
+ * 16-byte aligned; a call whose 128-position tiles over all sequences and kv
+ * heads could pass 2^31 is refused.  Two sequences must not append to the same
+ * page. */
 uint64_t strata_b200_tree_attention_workspace_bytes(int64_t tokens,
                                                     int64_t heads,
                                                     int64_t kv_heads,

@@ -364,7 +364,7 @@ def test_a_cache_that_runs_out_of_pages_stays_as_it_was(cuda, plugin, model):
                  pages_per_row=6)
     try:
         kv.fork([0, -1, -1, -1], reserve=60)
-        kv.lens[0] = 60
+        kv.lens[0] = 60  # of 64 positions
         before = kv.table.read()
         with pytest.raises(StrataError) as e:
             kv.fork([0, 0, 0, 0], reserve=1)
@@ -375,6 +375,8 @@ def test_a_cache_that_runs_out_of_pages_stays_as_it_was(cuda, plugin, model):
         assert e.value.code == -3
         with pytest.raises(ValueError):
             kv.accept([[1, 1], [], [], []])
+        with pytest.raises(ValueError):
+            kv.accept([[0, 4], [], [], []])  # the row has pages for 64 positions
         kv.fork([0, 0, -1, -1], reserve=0)
         assert kv.lens.tolist() == [60, 60, 0, 0]
     finally:
