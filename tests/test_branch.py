@@ -811,7 +811,8 @@ class Fork:
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("pages,ps,rows,per", [(40, 16, 5, 6), (9000, 16, 300, 9), (60, 64, 4, 5)])
+@pytest.mark.parametrize("pages,ps,rows,per", [(40, 16, 5, 6), (9000, 16, 300, 9), (60, 64, 4, 5), (1800, 16, 1100, 2),
+                                               (6000, 32, 1500, 3)])
 def test_kv_fork_from_a_prompt_through_beam_steps(cuda, lib, pages, ps, rows, per):
     """Grow one row, fan it out, then steps of random survivors and growth,
     ended rows and rows taken up again; every state equal to the definition's."""
