@@ -459,6 +459,64 @@ def test_tree_attention_in_graphs_and_on_two_streams(cuda, lib):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("page", [0, 64])
+def test_tree_attention_past_32_bit_offsets(cuda, lib, page):
+    """Caches of more than 2^31 elements: the last kv head's rows lie past every
+    32-bit offset.  Checked on the device in 64 bits, bound as in Tree.answer."""
+    torch = cuda
+    G, d, L, T = 16, 128, 1_100_032, 3
+    g = torch.Generator(device="cuda").manual_seed(5)
+    new = lambda *s: torch.randn(s, device="cuda", generator=g, dtype=torch.bfloat16)  # noqa: E731
+    kc, vc = (new(L // page, G, page, d) if page else new(1, G, L, d) for _ in range(2))
+    q, k, v = new(T, G * d), new(T, G * d), new(T, G * d)
+    at = L - 7
+    base = torch.tensor([at], dtype=torch.int32, device="cuda")
+    table = torch.arange(L // page - 1, -1, -1, dtype=torch.int32, device="cuda")[None].contiguous() if page else None
+    mask = torch.tensor([1, 3, 5], dtype=torch.int32, device="cuda")
+    ws = torch.empty(lib.strata_b200_tree_attention_workspace_bytes(T, G, G, d), dtype=torch.uint8, device="cuda")
+    out, status = torch.empty_like(q), torch.zeros(1, dtype=torch.int32, device="cuda")
+    assert kc.numel() > 2 ** 31
+    assert lib.strata_b200_tree_attention_bf16(
+        ptr(q), ptr(k), ptr(v), ptr(kc), ptr(vc), ptr(table), ptr(base), None, ptr(mask), 1, T, G, G, d, L, page,
+        L // page if page else 0, ptr(ws), ptr(out), ptr(status), torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    assert int(status.item()) == 0
+    for h in (0, G - 1):
+        rows = [(c.flip(0)[:, h] if page else c[0, h]).reshape(L, d)[:at + T] for c in (kc, vc)]
+        for r, x in zip(rows, (k, v)):
+            assert torch.equal(r[at:].view(torch.int16), x.view(T, G, d)[:, h].view(torch.int16))
+        s = rows[0].double() @ q.view(T, G, d)[:, h].double().T / d ** 0.5
+        s[at:][~torch.tensor([[1, 1, 1], [0, 1, 0], [0, 0, 1]], dtype=torch.bool, device="cuda")] = -np.inf
+        w = torch.softmax(s, 0).T
+        o, a = w @ rows[1].double(), w @ rows[1].double().abs()
+        off = (out.view(T, G, d)[:, h].double() - o).abs() - a * (2.0 ** -8 + 2.0 ** -12) - o.abs() * 2.0 ** -8
+        assert off.max().item() <= 0
+    if page:  # the same pool: a row forked, and an accepted path moved, near the pool's end
+        P = L // page
+        lens, parents = torch.tensor([70, 0], dtype=torch.int32, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
+        ti = torch.full((2, 3), -1, dtype=torch.int32, device="cuda")
+        ti[0, :2] = torch.tensor([P - 1, P - 2])
+        refs = torch.ones(P, dtype=torch.int32, device="cuda")
+        refs[P - 3] = 0  # the only free page
+        to, lo, ro = torch.empty_like(ti), torch.empty_like(lens), torch.empty_like(refs)
+        rep = torch.zeros(4, dtype=torch.int32, device="cuda")
+        fws = torch.empty(lib.strata_b200_kv_fork_workspace_bytes(2, 3, P), dtype=torch.uint8, device="cuda")
+        st = torch.cuda.current_stream().cuda_stream
+        assert lib.strata_b200_kv_fork(pools_array([kc]), 1, 2 * d, G, page, P, ptr(ti), ptr(lens), ptr(refs), ptr(parents),
+                                       2, 3, 1, ptr(to), ptr(lo), ptr(ro), ptr(rep), ptr(fws), st) == 0
+        torch.cuda.synchronize()
+        assert rep.tolist() == [0, 1, 0, 0] and to.tolist() == [[P - 1, P - 2, -1], [P - 1, P - 3, -1]]
+        assert torch.equal(kc[P - 3, :, :6].view(torch.int16), kc[P - 2, :, :6].view(torch.int16))
+        want = kc[P - 3, :, 9].clone()
+        nb, path, n = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, 70], [[0], [3]], [0, 1]))
+        assert lib.strata_b200_kv_accept(pools_array([kc]), 1, 2 * d, ptr(to), ptr(nb), ptr(path), ptr(n), 2, G, 3 * page,
+                                         1, page, P, ptr(status), st) == 0
+        torch.cuda.synchronize()
+        assert int(status.item()) == 0
+        assert torch.equal(kc[P - 3, :, 6].view(torch.int16), want.view(torch.int16))
+
+
+@pytest.mark.gpu
 def test_tree_attention_repeats_exactly(cuda, lib):
     torch = cuda
     t = Tree(31, 4, 31, 16, 2, 128, 3000, [2900, 1, 700, 2048])
