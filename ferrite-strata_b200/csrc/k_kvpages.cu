@@ -12,6 +12,14 @@
 // rows of 64 pools 9.9 us, most of it the plan's chain of dependent reads; 128 rows of
 // 32 pools 46 us, the copies alone (220 MB) 39 us with nothing cached, 5.6 TB/s;
 // compacting 3000 pages of 32 pools 240 us, the copies 236 us, 6.1 TB/s.
+//
+// What these kernels write, the decode attention may read before its wait (rows
+// below a position, the block table, positions).  So no later kernel may start
+// before it is written: the last kernel of each operator does not trigger its
+// dependents, which then start when it has ended.  And nothing that a kernel ahead
+// may write is read through const __restrict__ or __ldg here: either says that the
+// data stays as it is while the kernel runs, so the compiler may move such a load
+// above the wait.  (Block tables are: only the planning kernels write them.)
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -38,13 +46,12 @@ constexpr int kAcBatch = 8;  // rows in flight per thread
 // below every row a later group reads.  The moves with path[i] == i are a
 // prefix of the path and are skipped.
 __global__ void __launch_bounds__(kAcThreads)
-    kv_accept_kernel(const __grid_constant__ KvPools pools, int n_caches, int chunks, const int32_t* __restrict__ base,
-                     const int32_t* __restrict__ path, const int32_t* __restrict__ n_path, int kv_heads, int max_len,
-                     int max_path, KvPages kp, int* err) {
+    kv_accept_kernel(const __grid_constant__ KvPools pools, int n_caches, int chunks, const int32_t* base,
+                     const int32_t* path, const int32_t* n_path, int kv_heads, int max_len, int max_path, KvPages kp,
+                     int* err) {
   __shared__ int64_t s_src[kTreeMaxTokens], s_dst[kTreeMaxTokens];
   __shared__ int s_first;
-  pdl_trigger();
-  pdl_wait();
+  pdl_wait();  // no trigger: later kernels may read the rows before their own wait
   const int b = blockIdx.y;
   const int p0 = base[b], n = n_path[b];
   if (threadIdx.x == 0) s_first = n;
@@ -86,6 +93,7 @@ __global__ void __launch_bounds__(kAcThreads)
     for (int j = 0; j < kAcBatch; ++j)
       if (i0 + j < n) at[s_dst[i0 + j] * chunks] = v[j];
   }
+  __threadfence();
 }
 
 // ---------------------------------------------------------------------------
@@ -103,9 +111,8 @@ struct PageCopy {
 // [kv_heads, page_size, row]; a warp moves up to 4 KB of one head's rows.
 __global__ void __launch_bounds__(kCpThreads)
     page_copy_kernel(const __grid_constant__ KvPools pools, int n_pools, int kv_heads, int page_size, int chunks,
-                     const PageCopy* __restrict__ list, const int* __restrict__ n_list) {
-  pdl_trigger();
-  pdl_wait();
+                     const PageCopy* list, const int* n_list) {
+  pdl_wait();  // no trigger: later kernels may read the pages, and what the plan wrote, before their own wait
   const int lane = threadIdx.x & 31;
   const uint32_t pieces = uint32_t(page_size * chunks + kPiece - 1) / kPiece;
   const uint32_t per = uint32_t(n_pools) * uint32_t(kv_heads) * pieces;  // below 2^31 (launcher)
@@ -114,7 +121,8 @@ __global__ void __launch_bounds__(kCpThreads)
   // together a unit's number may pass 32 bits.
   uint32_t copy = first / per, in = first - copy * per;
   const uint32_t step_copy = warps / per, step_in = warps - step_copy * per;
-  const uint32_t copies = uint32_t(*n_list);
+  uint32_t copies;  // by a load that keeps its place behind the wait: the entries below it are then written, too
+  asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(copies) : "l"(n_list) : "memory");
   for (; copy < copies; copy += step_copy, in += step_in, copy += in >= per, in -= in >= per ? per : 0) {
     const PageCopy cp = list[copy];
     const uint32_t hp = in / pieces;
@@ -133,6 +141,7 @@ __global__ void __launch_bounds__(kCpThreads)
     for (int j = 0; j < kPiece / 32; ++j)
       if (c0 + j * 32 + lane < end) dst[j * 32] = v[j];
   }
+  __threadfence();
 }
 
 // ---------------------------------------------------------------------------
@@ -187,6 +196,7 @@ struct ForkArgs {
   const int32_t *table_in, *lens_in, *refs_in, *parents;
   int32_t *table_out, *lens_out, *refs_out, *report;
   int rows, per, page_shift, num_pages, reserve;
+  bool copies_follow;  // the copying kernel is launched behind the plan
   FastDiv by_per;
   // workspace; the first four in shared memory where one block plans
   int *left, *cand, *free_list, *row_off;
@@ -250,7 +260,7 @@ __global__ void __launch_bounds__(kPlThreads) kv_fork_plan_kernel(const __grid_c
     s_err = 0;
     s_low = 0;
   }
-  pdl_trigger();
+  if (a.copies_follow) pdl_trigger();
   pdl_wait();
 #pragma unroll 1
   for (int g = tid; g < a.num_pages; g += nthreads) {
@@ -398,6 +408,7 @@ __global__ void __launch_bounds__(kPlThreads) kv_fork_plan_kernel(const __grid_c
     a.report[2] = err ? 0 : total - copies;
     a.report[3] = err == kNoPages ? total - free_pages : err ? 0 : free_pages - total;
   }
+  __threadfence();
   cluster.sync();  // no block leaves while another may still read its shared memory
 }
 
@@ -405,6 +416,7 @@ struct CompactArgs {
   const int32_t *table_in, *refs_in;
   int32_t *table_out, *refs_out, *remap, *report;
   int rows, per, page_size, num_pages;
+  bool copies_follow;  // as in ForkArgs
   int* holes;
   PageCopy* copies;
   int* n_copies;
@@ -423,7 +435,7 @@ __global__ void __launch_bounds__(kPlThreads) kv_compact_plan_kernel(const Compa
     s_low = 0;
     s_err = 0;
   }
-  pdl_trigger();
+  if (a.copies_follow) pdl_trigger();
   pdl_wait();
   const int slice = (a.num_pages + nranks - 1) / nranks;
   const int run = (slice + kPlThreads - 1) / kPlThreads;
@@ -508,6 +520,7 @@ __global__ void __launch_bounds__(kPlThreads) kv_compact_plan_kernel(const Compa
     a.report[2] = moves;
     a.report[3] = err ? 0 : a.num_pages - n;
   }
+  __threadfence();
   cluster.sync();
 }
 
@@ -597,7 +610,7 @@ int launch_kv_fork(const KvPools& pools, int64_t n_pools, int64_t row_bytes, int
   if (units_per_copy(n_pools, row_bytes, kv_heads, page_size) > INT32_MAX) return SB_INVALID_ARGUMENT;
   ForkArgs a{table_in, lens_in, refs_in, parents, table_out, lens_out, refs_out, report, int(rows),
              int(pages_per_seq), __builtin_ctz(unsigned(page_size)), int(num_pages), int(reserve),
-             FastDiv(int(pages_per_seq)), nullptr, nullptr, nullptr, nullptr,
+             n_pools > 0, FastDiv(int(pages_per_seq)), nullptr, nullptr, nullptr, nullptr,
              nullptr, nullptr};
   Carve w{static_cast<uint8_t*>(workspace)};
   a.left = w.take<int>(uint64_t(num_pages));
@@ -629,7 +642,7 @@ int launch_kv_compact(const KvPools& pools, int64_t n_pools, int64_t row_bytes, 
                       void* workspace, cudaStream_t st) {
   if (units_per_copy(n_pools, row_bytes, kv_heads, page_size) > INT32_MAX) return SB_INVALID_ARGUMENT;
   CompactArgs a{table_in, refs_in, table_out, refs_out, remap, report, int(rows), int(pages_per_seq),
-                int(page_size), int(num_pages), nullptr, nullptr, nullptr};
+                int(page_size), int(num_pages), n_pools > 0, nullptr, nullptr, nullptr};
   Carve w{static_cast<uint8_t*>(workspace)};
   a.holes = w.take<int>(uint64_t(num_pages));
   a.copies = w.take<PageCopy>(uint64_t(num_pages));

@@ -1000,8 +1000,10 @@ constexpr int kJoinParts = 4;
 template <int D, bool Wide>
 __global__ void __launch_bounds__(128) tree_join_kernel(const Args a) {
   using L = Lay<D, Wide>;
-  pdl_trigger();
+  // Wait, then trigger: a kernel behind this one may read the cache before its own
+  // wait (the decode attention does), and the appended rows have to be there by then.
   pdl_wait();
+  pdl_trigger();
   const int c = int(blockIdx.x), row = int(threadIdx.x);
   const int t = Wide ? int(blockIdx.y) / (D / 8) : 0, col = int(blockIdx.y) % (D / 8);
   const Meta m = a.meta[c];
@@ -1118,7 +1120,7 @@ int launch(const TreeArgs& t, cudaStream_t st) {
                  vnm, a) != cudaSuccess)
     return SB_INTERNAL;
   count_launch();
-  if (grid == 1) return SB_OK;  // nothing is cut
+  // Also where nothing is cut: it holds later kernels back until the rows are appended.
   if (launch_pdl(tree_join_kernel<D, Wide>, dim3(grid, unsigned(D / 8 * (Wide ? 2 : 1))), dim3(128), 0, st, a) !=
       cudaSuccess)
     return SB_INTERNAL;

@@ -996,3 +996,115 @@ def test_kv_compact(cuda, lib, pages, live, rows):
     assert np.array_equal(to, np.where(table >= 0, remap[np.maximum(table, 0)], -1))
     for d, w in zip(dev, want):
         assert np.array_equal(d.cpu().numpy(), w)
+
+
+# ---------------------------------------------------------------------------
+# What one call writes is there for the next one on its stream
+# ---------------------------------------------------------------------------
+class DecodeAttention:
+    """Calls of the framework's decode attention, which reads cache rows below the position
+    before its wait for the kernel ahead of it."""
+
+    def __init__(self, torch, lib, B, H, G, d, L):
+        self.torch, self.lib, self.dims = torch, lib, (B, H, G, d, L)
+        lib.strata_b200_attention_decode_bf16.argtypes = [P] * 6 + [I64] * 5 + [P] * 3
+        lib.strata_b200_attention_decode_scratch_bytes.argtypes = [I64] * 4
+        lib.strata_b200_attention_decode_scratch_bytes.restype = C.c_uint64
+        new = lambda *s: torch.randn(s, device="cuda", generator=torch.Generator("cuda").manual_seed(s[-1]),  # noqa: E731
+                                     dtype=torch.bfloat16)
+        self.q, self.k, self.v = new(B, H * d), new(B, G * d), new(B, G * d)
+        self.scratch = torch.empty(lib.strata_b200_attention_decode_scratch_bytes(B, H, d, L), dtype=torch.uint8,
+                                   device="cuda")
+
+    def __call__(self, kc, vc, pos, out):
+        B, H, G, d, L = self.dims
+        assert self.lib.strata_b200_attention_decode_bf16(
+            ptr(self.q), ptr(self.k), ptr(self.v), ptr(kc), ptr(vc), ptr(pos), B, H, G, d, L, ptr(self.scratch), ptr(out),
+            self.torch.cuda.current_stream().cuda_stream) == 0
+
+
+def _back_to_back(torch, first, then, restore):
+    """Bits of `then()`'s outputs where the GPU is waited for between the two, and without, eagerly and in a graph."""
+    def go(between):
+        restore()
+        torch.cuda.synchronize()
+        first()
+        if between:
+            torch.cuda.synchronize()
+        outs = then()
+        torch.cuda.synchronize()
+        return [o.view(torch.int16).clone() for o in outs]
+
+    want = go(True)
+    for _ in range(10):
+        assert all(torch.equal(a, b) for a, b in zip(want, go(False)))
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        restore()
+        s.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            first()
+            outs = then()
+        for _ in range(5):
+            restore()
+            g.replay()
+            s.synchronize()
+            assert all(torch.equal(a, b.view(torch.int16)) for a, b in zip(want, outs))
+    return want
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("G,d", [(8, 128), (2, 64)])
+def test_decode_attention_right_behind_an_accept(cuda, lib, G, d):
+    """An accept moves rows of 64 caches, and the next step's attention over each of them is
+    launched at once: it reads the moved rows."""
+    torch = cuda
+    B, L, H, layers, width = 8, 320, 4 * G, 32, 40
+    rng = np.random.default_rng(G)
+    D = Dev(torch)
+    gen = torch.Generator("cuda").manual_seed(1)
+    init = torch.randn((2 * layers, B, G, L, d), device="cuda", generator=gen, dtype=torch.bfloat16)
+    caches = init.clone()
+    base = D(rng.integers(0, L - 2 * width, B).astype(np.int32))
+    path = D(np.stack([np.sort(rng.choice(2 * width, width, replace=False)) for _ in range(B)]).astype(np.int32))
+    n = D(np.full(B, width, np.int32))
+    pos = base + width  # the next token's position
+    attend = DecodeAttention(torch, lib, B, H, G, d, L)
+    outs = [torch.empty(B, H * d, dtype=torch.bfloat16, device="cuda") for _ in range(layers)]
+
+    def accept():
+        assert lib.strata_b200_kv_accept(pools_array(list(caches)), 2 * layers, 2 * d, None, ptr(base), ptr(path), ptr(n),
+                                         B, G, L, width, 0, 0, None, torch.cuda.current_stream().cuda_stream) == 0
+
+    def step():
+        for i in reversed(range(layers)):
+            attend(caches[2 * i], caches[2 * i + 1], pos, outs[i])
+        return outs
+
+    _back_to_back(torch, accept, step, lambda: caches.copy_(init))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,H,G,d", [(24, 32, 8, 128), (40, 8, 1, 64), (3, 4, 4, 128)])
+def test_decode_attention_right_behind_tree_attention(cuda, lib, T, H, G, d):
+    """The tree's rows are appended before a step behind it reads them."""
+    torch = cuda
+    B, L = 6, 640
+    t = Tree(T, B, T, H, G, d, L, [500, 3, 0, 129, 600 - T, 255])
+    s = t.call(torch, lib)
+    torch.cuda.synchronize()
+    init = [torch.from_numpy(x.view(np.int16)).cuda() for x in (t.kc, t.vc)]
+    pos = s["base"] + T
+    attend = DecodeAttention(torch, lib, B, H, G, d, L)
+    out = torch.empty(B, H * d, dtype=torch.bfloat16, device="cuda")
+
+    def restore():
+        s["kc"].copy_(init[0])
+        s["vc"].copy_(init[1])
+
+    def step():
+        attend(s["kc"], s["vc"], pos, out)
+        return [out]
+
+    _back_to_back(torch, lambda: t.call(torch, lib, state=s), step, restore)

@@ -6,6 +6,8 @@ On the CPU the oracle's tree step must equal sequential decode steps along every
 branch.  On the GPU the graphs are compared with the oracle, a speculative loop
 with plain greedy decoding, and a beam search with one that re-reads every beam
 from its prompt."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -381,3 +383,88 @@ def test_a_cache_that_runs_out_of_pages_stays_as_it_was(cuda, plugin, model):
         assert kv.lens.tolist() == [60, 60, 0, 0]
     finally:
         kv.release()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op", ["fork", "fork of the table alone", "compact"])
+def test_a_step_right_behind_a_page_operation(cuda, plugin, op):
+    """A decode attention graph launched behind a fork or a compaction, without a wait in between,
+    reads the new table, lengths and pages."""
+    torch = cuda
+    rng = np.random.default_rng(9)
+    R, per, ps, G, H, d, pools = 96, 12, 16, 2, 8, 128, 16
+    pages = R * per + 200
+    lib, stream = plugin.lib, plugin.stream()
+    dev = lambda x: torch.from_numpy(np.ascontiguousarray(x)).cuda()  # noqa: E731
+    i32 = lambda *s: torch.full(s, -5, dtype=torch.int32, device="cuda")  # noqa: E731
+    lens = rng.integers(1, (per - 1) * ps, R).astype(np.int32)
+    ids, table, at = rng.permutation(pages).astype(np.int32), np.full((R, per), -1, np.int32), 0
+    for r in range(R):
+        n = -(-int(lens[r] + 1) // ps)
+        table[r, :n] = ids[at:at + n]
+        at += n
+    refs = np.zeros(pages, np.int32)
+    refs[ids[:at]] = 1
+    init = torch.randn((pools, pages, G, ps, d), device="cuda", dtype=torch.bfloat16)
+    pool = init.clone()
+    ti, li, ri, pa = dev(table), dev(lens), dev(refs), dev(rng.integers(0, R, R).astype(np.int32))
+    to, lo, ro, remap, report = i32(R, per), i32(R), i32(pages), i32(pages), i32(4)
+    n_pools = 0 if "alone" in op else pools
+    ptrs = (ctypes.c_void_p * pools)(*[p.data_ptr() for p in pool])
+    P, I64 = ctypes.c_void_p, ctypes.c_int64
+    lib.strata_b200_kv_fork_workspace_bytes.restype = lib.strata_b200_kv_compact_workspace_bytes.restype = ctypes.c_uint64
+    lib.strata_b200_kv_fork_workspace_bytes.argtypes = [I64] * 3
+    lib.strata_b200_kv_compact_workspace_bytes.argtypes = [I64]
+    ws = torch.empty(max(lib.strata_b200_kv_fork_workspace_bytes(R, per, pages),
+                         lib.strata_b200_kv_compact_workspace_bytes(pages)), dtype=torch.uint8, device="cuda")
+    lib.strata_b200_kv_fork.argtypes = [P] + [I64] * 5 + [P] * 4 + [I64] * 3 + [P] * 6
+    lib.strata_b200_kv_compact.argtypes = [P] + [I64] * 5 + [P] * 2 + [I64] * 2 + [P] * 6
+
+    def page_op():
+        if op == "compact":
+            return lib.strata_b200_kv_compact(ptrs, n_pools, 2 * d, G, ps, pages, ti.data_ptr(), ri.data_ptr(), R, per,
+                                              to.data_ptr(), ro.data_ptr(), remap.data_ptr(), report.data_ptr(),
+                                              ws.data_ptr(), stream)
+        return lib.strata_b200_kv_fork(ptrs, n_pools, 2 * d, G, ps, pages, ti.data_ptr(), li.data_ptr(), ri.data_ptr(),
+                                       pa.data_ptr(), R, per, 1, to.data_ptr(), lo.data_ptr(), ro.data_ptr(),
+                                       report.data_ptr(), ws.data_ptr(), stream)
+
+    b = GraphBuilder("t")
+    q, k, v = (b.input(BF16, (R, n * d), x) for n, x in ((H, "q"), (G, "k"), (G, "v")))
+    kc, vc = (b.input(BF16, (pages, G, ps, d), x) for x in ("kc", "vc"))
+    pos, tab = b.input(I32, (R,), "pos"), b.input(I32, (R, per), "table")
+    outs = b.node(Op.custom("fused::attention"), [q, k, v, kc, vc, pos, tab], [(BF16, (R, H * d))],
+                  {"num_heads": H, "num_kv_heads": G, "head_dim": d, "page_size": ps}, "a")
+    b.output(outs[0])
+    g = b.build()
+    new = [torch.randn((R, n * d), device="cuda", dtype=torch.bfloat16) for n in (H, G, G)]
+    out = torch.empty((R, H * d), device="cuda", dtype=torch.bfloat16)
+    where = {q: new[0], k: new[1], v: new[2], kc: pool[-2], vc: pool[-1], pos: li if op == "compact" else lo, tab: to,
+             outs[0]: out}
+    bufs = {i: plugin.wrap(t.data_ptr(), t.numel() * t.element_size()) for i, t in where.items()}
+
+    def go(wait):
+        pool.copy_(init)
+        for x in (to, lo):
+            x.fill_(0)
+        torch.cuda.synchronize()
+        exe = plugin.compile(g)  # a new one: its first run is not a captured one
+        run = exe.bind({i: Device(x) for i, x in bufs.items()})
+        try:
+            assert page_op() == 0
+            if wait:
+                torch.cuda.synchronize()
+            run.run_async()
+            plugin.synchronize()
+            assert report[0].item() == 0 and report[1].item() > 0
+            return out.view(torch.int16).clone()
+        finally:
+            run.release()
+            exe.free()
+
+    want = go(True)
+    assert want.any()
+    for _ in range(10):
+        assert torch.equal(want, go(False))
+    for x in bufs.values():
+        x.release()
