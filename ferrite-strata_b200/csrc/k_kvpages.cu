@@ -236,7 +236,8 @@ __device__ __forceinline__ ForkRow fork_row(const ForkArgs& a, int r) {
 
 // One cluster plans the whole call.  left[g] counts the references to page g
 // that remain when the old table lets go and every row has taken its parent's
-// full pages; integer atomics, so the order of the threads does not matter.
+// full pages, first the one and then the other; integer atomics, so the order of
+// the threads does not matter.
 // A partly filled page with left[g] == 0 stays with the lowest row that wants
 // it (cand[g]), everyone else gets a copy.  A page is free when nobody holds
 // or wants it; the free pages are dealt out in ascending order to the rows in
@@ -270,27 +271,25 @@ __global__ void __launch_bounds__(kPlThreads) kv_fork_plan_kernel(const __grid_c
   cluster.sync();
   int err = 0;
   const int entries = a.rows * a.per;
+  // The old table lets go of everything before the new one takes anything: a count
+  // below the old references would not show among the new ones.
+#pragma unroll 1
+  for (int e = tid; e < entries; e += nthreads) {
+    const int old = a.table_in[e];
+    if (old >= a.num_pages) err = max(err, kBadPage);
+    else if (old >= 0 && atomicSub(&a.left[old], 1) <= 0) err = max(err, kBadRefs);
+  }
+  cluster.sync();
 #pragma unroll 1
   for (int e = tid; e < entries; e += nthreads) {
     const int r = a.by_per.div(e), i = e - r * a.per;
-    const int old = a.table_in[e];
-    if (old >= a.num_pages) err = max(err, kBadPage);
     const ForkRow f = fork_row(a, r);
     if (f.bad) err = max(err, kBadPosition);
-    int mine = -1;
-    if (f.parent >= 0 && (i < f.full || (i == f.full && f.part))) {
-      mine = f.parent == r ? old : a.table_in[f.parent * a.per + i];
-      if (mine < 0 || mine >= a.num_pages) {
-        err = max(err, kBadPage);
-        mine = -1;
-      }
-    }
-    const bool shares = mine >= 0 && i < f.full;
-    if (!(shares && mine == old)) {  // otherwise one reference goes and one comes
-      if (old >= 0 && old < a.num_pages) atomicSub(&a.left[old], 1);
-      if (shares) atomicAdd(&a.left[mine], 1);
-    }
-    if (mine >= 0 && i == f.full) atomicMin(&a.cand[mine], r);
+    if (f.parent < 0 || i > f.full || (i == f.full && !f.part)) continue;
+    const int mine = a.table_in[f.parent * a.per + i];
+    if (mine < 0 || mine >= a.num_pages) err = max(err, kBadPage);
+    else if (i < f.full) atomicAdd(&a.left[mine], 1);
+    else atomicMin(&a.cand[mine], r);
   }
   if (err) atomicMax(&s_err, err);
   cluster.sync();

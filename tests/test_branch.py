@@ -1108,3 +1108,33 @@ def test_decode_attention_right_behind_tree_attention(cuda, lib, T, H, G, d):
         return [out]
 
     _back_to_back(torch, lambda: t.call(torch, lib, state=s), step, restore)
+
+
+def _under_counted(case):
+    """(pages, rows, per, table, lens, refs, parents) whose counts are below the table's own references."""
+    if case == "one row keeps the page, another lets it go":
+        return 4, 2, 2, [[0, -1], [0, -1]], [16, 16], [1, 0, 0, 0], [0, -1]
+    if case == "a page without a reference is shared out":
+        return 3, 2, 2, [[0, 1], [-1, -1]], [32, 0], [0, 1, 0], [0, 0]
+    if case == "every row keeps it":
+        return 3, 3, 1, [[2], [2], [2]], [16] * 3, [0, 0, 2], [0, 1, 2]
+    if case == "a row takes it from another that keeps it":
+        return 3, 3, 2, [[2, -1], [1, 2], [-1, -1]], [16, 32, 0], [0, 1, 1], [0, 0, 1]
+    # planned by a cluster: one reference is missing among many
+    return 5000, 1100, 2, [[7, -1]] * 1100, [16] * 1100, [1099 if g == 7 else 0 for g in range(5000)], \
+        [r if r % 3 else (r * 7) % 1100 for r in range(1100)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", ["one row keeps the page, another lets it go", "a page without a reference is shared out",
+                                  "every row keeps it", "a row takes it from another that keeps it", "many rows"])
+def test_kv_fork_counts_the_old_references_before_the_new_ones(cuda, lib, case):
+    """Error 3 compares the counts with the old table, whatever the new one shares: an
+    under-counted page must not come out free beside a row that holds it."""
+    pages, rows, per, table, lens, refs, parents = _under_counted(case)
+    f = Fork(cuda, lib, pages, 16, rows, per, pools=1)
+    f.table[:], f.lens[:], f.refs[:] = table, lens, refs
+    assert f.step(parents, reserve=0)[0] == 3
+    named = f.table[f.table >= 0]
+    f.refs = np.bincount(named, minlength=pages).astype(np.int32)  # with all references counted it goes through
+    assert f.step(parents, reserve=0)[0] == 0
