@@ -16,7 +16,8 @@
 // What these kernels write, the decode attention may read before its wait (rows
 // below a position, the block table, positions).  So no later kernel may start
 // before it is written: the last kernel of each operator does not trigger its
-// dependents, which then start when it has ended.  And nothing that a kernel ahead
+// dependents, which then start when it has ended, and its writes are fenced, since the
+// end of a kernel is not yet the end of its writes for one that starts early.  And nothing that a kernel ahead
 // may write is read through const __restrict__ or __ldg here: either says that the
 // data stays as it is while the kernel runs, so the compiler may move such a load
 // above the wait.  (Block tables are: only the planning kernels write them.)
@@ -80,11 +81,12 @@ __global__ void __launch_bounds__(kAcThreads)
   const int64_t u = int64_t(blockIdx.x) * kAcThreads + threadIdx.x;
   const int c = int(u % chunks);
   const int64_t ch = u / chunks;
-  const int h = int(ch % kv_heads), cache = int(ch / kv_heads);
-  if (cache >= n_caches) return;
+  const int h = int(ch % kv_heads);
+  const int64_t cache = ch / kv_heads;
+  const bool on = cache < n_caches;  // the last block may reach past the last cache
   const int64_t head_rows = int64_t(h) * (kp.paged() ? kp.page_size : max_len);
-  uint4* at = static_cast<uint4*>(pools.p[cache]) + head_rows * chunks + c;
-  for (int i0 = first; i0 < n; i0 += kAcBatch) {
+  uint4* at = static_cast<uint4*>(pools.p[on ? cache : 0]) + head_rows * chunks + c;
+  for (int i0 = on ? first : n; i0 < n; i0 += kAcBatch) {
     uint4 v[kAcBatch];
 #pragma unroll
     for (int j = 0; j < kAcBatch; ++j)
@@ -93,7 +95,9 @@ __global__ void __launch_bounds__(kAcThreads)
     for (int j = 0; j < kAcBatch; ++j)
       if (i0 + j < n) at[s_dst[i0 + j] * chunks] = v[j];
   }
-  __threadfence();
+  // One fence for the block's rows; by each thread it cost another 1.1 us of 17.6 (32 paths, 160 pools).
+  __syncthreads();
+  if (threadIdx.x == 0) __threadfence();
 }
 
 // ---------------------------------------------------------------------------
@@ -149,6 +153,7 @@ __global__ void __launch_bounds__(kCpThreads)
 // ---------------------------------------------------------------------------
 constexpr int kPlThreads = 1024;
 constexpr int kPlMaxCluster = 8;
+static_assert(kPlThreads * kPlMaxCluster <= kPlanStep, "indexes of table entries stay below 2^31");
 constexpr int kPlItems = 4 * kPlThreads;  // table entries and pages that one block plans alone
 
 // Division of numbers below 2^31 by a fixed positive one: floor(n m / 2^(31 + s))
