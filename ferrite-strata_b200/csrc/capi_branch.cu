@@ -129,7 +129,7 @@ static bool pool_args(void* const* pools, int64_t n_pools, int64_t row_bytes, in
   return make_pools(pools, n_pools, row_bytes, p) && fits(kv_heads, 1, 65535) && kv_page_size_ok(page_size) &&
          fits(num_pages, 1, INT32_MAX / 2) && num_pages <= INT32_MAX / kv_heads / page_size && fits(rows, 0, 65536) &&
          fits(pages_per_seq, 1) && pages_per_seq <= INT32_MAX / page_size &&
-         rows * pages_per_seq <= INT32_MAX;
+         rows * pages_per_seq <= INT32_MAX - kPlanStep;
 }
 
 uint64_t strata_b200_kv_fork_workspace_bytes(int64_t rows, int64_t pages_per_seq, int64_t num_pages) {

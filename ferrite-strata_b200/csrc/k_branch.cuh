@@ -50,6 +50,8 @@ struct KvPools {
 int launch_kv_accept(const KvPools& caches, int64_t n_caches, int64_t row_bytes, const int32_t* base,
                      const int32_t* path, const int32_t* n_path, int64_t batch, int64_t kv_heads, int64_t max_len,
                      int64_t max_path, const KvPages& kp, int* err, cudaStream_t st);
+// Table entries that a planning kernel steps over at once; a table ends that far below 2^31.
+constexpr int kPlanStep = 8192;
 uint64_t kv_fork_workspace_bytes(int64_t rows, int64_t pages_per_seq, int64_t num_pages);
 int launch_kv_fork(const KvPools& pools, int64_t n_pools, int64_t row_bytes, int64_t kv_heads, int64_t page_size,
                    int64_t num_pages, const int32_t* table_in, const int32_t* lens_in, const int32_t* refs_in,

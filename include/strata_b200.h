@@ -294,7 +294,8 @@ int32_t strata_b200_kv_accept(
  * the row), 3 refs below the table's references, 5 too few free pages (report
  * [3] is how many more are needed), 6 a needed entry that names no page; the
  * outputs are then copies of the inputs and the pools are not touched.
- * rows <= 65536; a call with no rows writes nothing. */
+ * rows <= 65536, rows * pages_per_seq < 2^31 - 8192; a call with no rows writes
+ * nothing. */
 uint64_t strata_b200_kv_fork_workspace_bytes(int64_t rows,
                                              int64_t pages_per_seq,
                                              int64_t num_pages);

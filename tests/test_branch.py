@@ -162,6 +162,20 @@ def test_kv_compact_refuses(hlib, bad):
     assert hlib.strata_b200_kv_compact(*a.values()) == INVALID
 
 
+@pytest.mark.parametrize("entry", ["strata_b200_kv_fork", "strata_b200_kv_compact"])
+def test_tables_that_a_32_bit_index_cannot_step_over_are_refused(hlib, entry):
+    """The planning kernels step through the table by up to 8192 entries, so a table that ends
+    closer than that to 2^31 is refused; so is one past it."""
+    tail = dict(l_in=X, r_in=X, par=X) if entry.endswith("fork") else dict(r_in=X)
+    for rows, per in ((16, (1 << 27) - 1), (65536, 1 << 15), (32765, 65542)):
+        a = dict(pools=(P * 2)(X, X), n=2, row=256, heads=2, page=16, pages=8, t_in=X, **tail, rows=rows, per=per)
+        if entry.endswith("fork"):
+            a.update(reserve=1, t_out=2 * X, l_out=2 * X, r_out=2 * X, rep=2 * X, ws=X, stream=None)
+        else:
+            a.update(t_out=2 * X, r_out=2 * X, remap=3 * X, rep=2 * X, ws=X, stream=None)
+        assert getattr(hlib, entry)(*a.values()) == INVALID
+
+
 # ---------------------------------------------------------------------------
 # tree attention
 # ---------------------------------------------------------------------------
