@@ -825,7 +825,11 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int c = 0; c < 4; ++c)
                 mc[c] = fmax3(mc[c], __uint_as_float(r[e + 2 * c]), __uint_as_float(r[e + 2 * c + 1]));
             float mt = fmaxf(fmaxf(mc[0], mc[1]), fmaxf(mc[2], mc[3])) * sl;
-            if (pair_any(pair_bar, mt > m_ref + kRescale)) {  // also the first tile with anything to see
+            // The vote also stands between this thread's read of S and the other's P in its columns.
+            tc_fence_before();
+            const bool moves = pair_any(pair_bar, mt > m_ref + kRescale);
+            tc_fence_after();
+            if (moves) {  // also the first tile with anything to see
               // Both threads of a row take the larger maximum: exchanged in two
               // columns of S, which both have read.
               tmem_st1(tS + uint32_t(kHalf + half), __float_as_uint(mt));
