@@ -222,6 +222,14 @@ __device__ __forceinline__ void prefetch_l2(const uint4* p, int n) {
   asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(n * 16) : "memory");
 }
 
+// Logits come from the kernel ahead, which may run when this one starts: their
+// loads keep their place behind the wait, which __ldg does not promise.
+__device__ __forceinline__ uint4 ld_logits(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
 // N is 1 for lists of 32 (keep <= 32), 2 for lists of 64.
 template <typename T, int N>
 __global__ void __launch_bounds__(kThreads) beam_run_kernel(const BeamArgs<T> a) {
@@ -264,13 +272,13 @@ __global__ void __launch_bounds__(kThreads) beam_run_kernel(const BeamArgs<T> a)
     if (lane == 0 && t0 + 2 * kTile < v1) prefetch_l2(blocks + ahead, min(kStep / kVec, last_block + 1 - ahead));
     if (mis == 0) {
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) u[i] = __ldg(blocks + min(blk + i * 32, last_block));
+      for (int i = 0; i < kLoads; ++i) u[i] = ld_logits(blocks + min(blk + i * 32, last_block));
     } else {
       uint4 hi[kLoads];
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
-        u[i] = __ldg(blocks + min(blk + i * 32, last_block));
-        hi[i] = __ldg(blocks + min(blk + i * 32 + 1, last_block));
+        u[i] = ld_logits(blocks + min(blk + i * 32, last_block));
+        hi[i] = ld_logits(blocks + min(blk + i * 32 + 1, last_block));
       }
       const uint32_t sh = (mis & 2) * 8;
 #pragma unroll
