@@ -249,7 +249,8 @@ int32_t strata_b200_tree_attention_bf16(
  * [batch, keep].  Where no candidate above -inf is left: -inf, -1, -1, 0.
  * eos -1: no token ends a beam (an ended beam's token is then -1).  keep <=
  * 64, beams <= 1024, batch * beams <= 65535, vocab <= 2^30.  Scores are added
- * and compared in f64 and rounded once; the softmax's terms are f32. */
+ * and compared in f64 and rounded once; the softmax's terms are f32, and the
+ * logarithm of their sum is within 2^-20. */
 uint64_t strata_b200_beam_select_workspace_bytes(int64_t batch, int64_t beams,
                                                  int64_t vocab, int64_t keep);
 int32_t strata_b200_beam_select_bf16(

@@ -703,6 +703,38 @@ def test_beam_select_in_a_graph(cuda, lib):
     assert np.array_equal(outs[2].cpu().numpy().reshape(2, 4), want[2])
 
 
+def _hard_pairs(rng, lo, hi, n, half):
+    """n pairs (a, x), x - a in [lo, hi], for which (x - a) log2(e) in f32 is farthest from the
+    exact product, so 2^it from exp(x - a)."""
+    a = rng.uniform(-3, 3, 200 * n).astype(np.float32)
+    x = (a + rng.uniform(lo, hi, a.size)).astype(np.float32)
+    if half:
+        a, x = ora.round_bf16(a), ora.round_bf16(x)
+    d = x.astype(np.float64) - a
+    e = (x - a).astype(np.float32) * np.float32(1.4426950408889634)
+    off = np.where((d >= lo) & (d <= hi), np.abs(e.astype(np.float64) - d * 1.4426950408889634074), -1.0)
+    order = np.argsort(-off)[:n]
+    rng.shuffle(order)
+    return a[order], x[order]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("lo,hi", [(0.5, 2.0), (2.0, 4.0), (4.0, 8.0), (11.1, 15.99), (15.99, 40.0)])
+def test_beam_select_a_logit_far_above_the_ones_before(cuda, lib, lo, hi, half):
+    """Two logits a row, which one thread meets in turn, the larger one last: the sum of
+    exponentials keeps its bound however far the second lies above the first."""
+    rng = np.random.default_rng(int(lo * 100) + half)
+    batch, beams, vocab = 8, 32, 32768
+    a, x = _hard_pairs(rng, lo, hi, batch * beams, half)
+    rows = np.full((batch * beams, vocab), -np.inf, np.float32)
+    for r in range(batch * beams):
+        at = int(rng.integers(0, 8)) * 1024 + int(rng.integers(0, 32)) * (8 if half else 4)
+        rows[r, at], rows[r, at + 8192] = a[r], x[r]
+    scores = np.log1p(np.exp(a.astype(np.float64) - x)) - np.tile(np.arange(beams) * 2.0 ** -10, batch)  # a step apart
+    beam_check(cuda, lib, bf(rows) if half else rows, scores, None, batch, beams, beams, -1)
+
+
 # ---------------------------------------------------------------------------
 # kv_accept
 # ---------------------------------------------------------------------------
