@@ -140,6 +140,39 @@ class PagedKv:
         self.held = np.where(parents >= 0, pages * self.page_size, 0)
         return report
 
+    def reserve(self, need) -> None:
+        """Gives each row free pages for ``need[r]`` positions past its length, the lowest ids first, to
+        rows in ascending order; a row that has them keeps its pages.  A row's partly filled page has
+        to be its own, as a fork leaves it.  On an error the rows stay as they were."""
+        need = np.asarray(need, np.int64)
+        if need.shape != (self.rows,) or (need < 0).any():
+            raise ValueError("one number of positions per row")
+        want = -(-(self.lens + need) // self.page_size)
+        if (want > self.pages_per_row).any():
+            raise StrataError(abi.INVALID_ARGUMENT, "reserve: a row would pass its last page")
+        for attempt in range(2):
+            have = self.held // self.page_size
+            more = np.maximum(want - have, 0)
+            if not more.any():
+                return
+            refs = np.frombuffer(self._refs[self.side].read(), np.int32).copy()
+            free = np.flatnonzero(refs == 0)
+            if more.sum() <= free.size:
+                break
+            if attempt:
+                raise StrataError(abi.RESOURCE_EXHAUSTED, "reserve: the pool has too few free pages "
+                                                          f"({more.sum() - free.size} more are needed)")
+            self.fork(np.arange(self.rows), reserve=0)  # what rows hold past their lengths goes back
+        table = np.frombuffer(self.table.read(), np.int32).reshape(self.rows, self.pages_per_row).copy()
+        at = 0
+        for r in np.flatnonzero(more):
+            table[r, have[r]:want[r]] = free[at:at + more[r]]
+            at += more[r]
+        refs[free[:at]] = 1
+        self.table.write(table)
+        self._refs[self.side].write(refs)
+        self.held = np.maximum(self.held, want * self.page_size)
+
     def compact(self) -> np.ndarray:
         """Moves the used pages to the lowest ids; returns [0, pages used, pages moved, pages free]."""
         a, b = self.side, 1 - self.side
@@ -225,9 +258,7 @@ class _Decoder:
         kv.fork(np.full(kv.rows, -1), reserve=0)
         if not prompts:
             return
-        # Empty rows that continue themselves get the pages the reservation asks for;
-        # what a shorter prompt does not fill goes back with the next fork.
-        kv.fork([r if r in prompts else -1 for r in range(kv.rows)], reserve=max(map(len, prompts.values())))
+        kv.reserve([len(prompts.get(r, ())) for r in range(kv.rows)])
         for row, tokens in prompts.items():
             n = len(tokens)
             g, hd = self._graph(batch=1, seq=n, head="none")

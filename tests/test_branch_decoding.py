@@ -468,3 +468,75 @@ def test_a_step_right_behind_a_page_operation(cuda, plugin, op):
         assert torch.equal(want, go(False))
     for x in bufs.values():
         x.release()
+
+
+@pytest.mark.gpu
+def test_reserve_gives_each_row_its_pages(cuda, plugin):
+    """Lowest free ids first, nothing for rows that have enough, and pages past a row's length
+    taken back only when the pool is short."""
+    kv = PagedKv(plugin, pools=2, pages=8, kv_heads=1, page_size=16, head_dim=64, rows=3, pages_per_row=4)
+
+    def state():
+        table = np.frombuffer(kv.table.read(), np.int32).reshape(3, 4).tolist()
+        refs = np.frombuffer(kv._refs[kv.side].read(), np.int32).tolist()
+        ids = [g for row in table for g in row if g >= 0]
+        assert refs == [ids.count(g) for g in range(8)]
+        assert kv.held.tolist() == [16 * sum(g >= 0 for g in row) for row in table]
+        return [[g for g in row if g >= 0] for row in table]
+
+    try:
+        kv.reserve([17, 0, 1])
+        assert state() == [[0, 1], [], [2]]
+        kv.lens[:] = [5, 0, 16]
+        kv.reserve([27, 0, 0])
+        assert state() == [[0, 1], [], [2]]
+        kv.reserve([0, 33, 1])
+        assert state() == [[0, 1], [3, 4, 5], [2, 6]]
+        with pytest.raises(StrataError) as e:
+            kv.reserve([60, 0, 0])  # past the row
+        assert e.value.code == -3 and state() == [[0, 1], [3, 4, 5], [2, 6]]
+        kv.lens[1] = 33
+        kv.reserve([0, 0, 32])
+        assert state() == [[0, 1], [3, 4, 5], [2, 6, 7]]
+        kv.reserve([43, 15, 0])  # no page is free: rows 0 and 2 let go of those they do not fill
+        assert state() == [[0, 1, 6], [3, 4, 5], [2]]
+        kv.reserve([43, 16, 0])
+        assert state() == [[0, 1, 6], [3, 4, 5, 7], [2]]
+        with pytest.raises(StrataError) as e:
+            kv.reserve([59, 0, 17])
+        assert e.value.code == -5 and "(2 more are needed)" in str(e.value)
+        assert state() == [[0], [3, 4, 5], [2]] and kv.lens.tolist() == [5, 33, 16]
+        for bad in ([1, 1], [1, -1, 0]):
+            with pytest.raises(ValueError):
+                kv.reserve(bad)
+    finally:
+        kv.release()
+
+
+@pytest.mark.gpu
+def test_a_ragged_prefill_needs_only_its_prompts_pages(cuda, plugin, model):
+    """One long prompt beside short ones in a pool that holds them and one step, not the longest
+    length for every row; the step then continues each prompt."""
+    rng = np.random.default_rng(5)
+    prompts = [[int(x) for x in rng.integers(0, 300, n)] for n in (7, 81, 3, 2)]  # 1 + 5 + 1 + 1 pages cached
+    kv = PagedKv(plugin, pools=2 * SMALL.layers, pages=9, kv_heads=2, page_size=16, head_dim=64, rows=4,
+                 pages_per_row=8)
+    dec = TreeDecoder(plugin, SMALL, model.weights, kv, nodes=2)
+    try:
+        dec.start(prompts)
+        assert kv.lens.tolist() == [6, 80, 2, 1]
+        got = dec.step([([], [])] * 4)
+        for p, g in zip(prompts, got):
+            x = model.logits(p)
+            assert len(g) == 1 and (g[0] == int(np.argmax(x)) or _gap(x) < 0.02)
+        with pytest.raises(StrataError) as e:
+            dec.start([prompts[1], prompts[1], [1], [1]])  # 5 + 5 pages of 9
+        assert e.value.code == -5 and "1 more" in str(e.value)
+        with pytest.raises(StrataError) as e:
+            dec.start([[1] * 130, [1], [1], [1]])  # 129 of 128 positions
+        assert e.value.code == -3
+        dec.start(prompts)
+        assert kv.lens.tolist() == [6, 80, 2, 1]
+    finally:
+        dec.release()
+        kv.release()
