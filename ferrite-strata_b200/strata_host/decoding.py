@@ -3,8 +3,8 @@
 ``PagedKv`` owns the page pools of every layer with their block table, lengths
 and reference counts, and drives the page operations of include/strata_b200.h
 (``kv_fork``, ``kv_compact``, ``kv_accept``) on the plugin's stream.
-``BeamDecoder`` runs beam-search steps: one decoder graph with the beam head,
-then a fork of the cache by the chosen parents.  ``TreeDecoder`` runs drafted-tree
+``BeamDecoder`` runs beam-search steps: a fork of the cache by the parents chosen
+before, then one decoder graph with the beam head.  ``TreeDecoder`` runs drafted-tree
 steps: one graph that scores every node, the longest branch the argmax agrees
 with, then the accepted rows kept in place.
 
@@ -291,7 +291,11 @@ class _Decoder:
 
 class BeamDecoder(_Decoder):
     """Beam search of ``sentences`` prompts with ``beams`` beams each: the kv cache has one row
-    per beam, and sentence s's beams are rows s * beams, ..."""
+    per beam, and sentence s's beams are rows s * beams, ...
+
+    A step first gives every row the parent that the step before chose and room for its
+    token, so the cache follows a choice when the next step starts, and a step that
+    fills the rows still returns.  Ended beams take a position a step like the others."""
 
     def __init__(self, plugin: Plugin, shape: DecoderShape, weights: dict, kv: PagedKv, *, sentences: int, beams: int,
                  eos: int = -1, fmt: str = "w4g32", layers: int | None = None):
@@ -318,6 +322,7 @@ class BeamDecoder(_Decoder):
                 self._runs[side, cur] = exe.bind(arena)
         self._bound = list(self._runs.values())
         self._cur = 0
+        self._next = np.arange(R)  # each row's parent at the next step
         self.tokens = self.parents = self.scores = self.done = None
 
     def start(self, prompts) -> None:
@@ -327,7 +332,7 @@ class BeamDecoder(_Decoder):
             raise ValueError("one prompt of at least one token per sentence")
         self.prefill({s * W: p[:-1] for s, p in enumerate(prompts)})
         last = [int(p[-1]) for p in prompts for _ in range(W)]
-        kv.fork([s * W for s in range(self.sentences) for _ in range(W)], reserve=1)
+        self._next = np.repeat(np.arange(self.sentences) * W, W)
         scores = np.where(np.arange(kv.rows) % W == 0, 0.0, -np.inf).astype(np.float32)  # the beams are equal: one counts
         s, t, d = self._state[self._cur]
         s.write(scores)
@@ -336,8 +341,11 @@ class BeamDecoder(_Decoder):
 
     def step(self):
         """One step of every beam: (scores, parent rows, tokens, done), each [sentences, beams].
-        After an error the search has to start again."""
+        Where the rows or the pool have no room for it, nothing changes; after another error the
+        search has to start again."""
         kv = self.kv
+        kv.fork(self._next, reserve=1)
+        self._next = np.arange(kv.rows)
         self._pos.write(kv.lens)
         self._runs[kv.side, self._cur].run()
         self._cur = 1 - self._cur
@@ -349,7 +357,7 @@ class BeamDecoder(_Decoder):
         if (self.parents < 0).any():
             raise StrataError(abi.INVALID_ARGUMENT, "a sentence has fewer continuations than beams")
         kv.lens = kv.lens + 1
-        kv.fork(self.parents.reshape(-1), reserve=1)
+        self._next = self.parents.reshape(-1)
         return self.scores, self.parents, self.tokens, self.done
 
     def search(self, prompts, steps: int):

@@ -540,3 +540,38 @@ def test_a_ragged_prefill_needs_only_its_prompts_pages(cuda, plugin, model):
     finally:
         dec.release()
         kv.release()
+
+
+@pytest.mark.gpu
+def test_a_beam_search_goes_to_its_rows_end(cuda, plugin, model):
+    """The step that fills the rows returns its results; the next one is refused and the
+    cache and the beams stay as they were."""
+    W = 3
+    prompt = [int(x) for x in np.random.default_rng(6).integers(0, 300, 12)]
+    long, short = (PagedKv(plugin, pools=2 * SMALL.layers, pages=40, kv_heads=2, page_size=16, head_dim=64, rows=W,
+                           pages_per_row=n) for n in (4, 1))
+    a, b = (BeamDecoder(plugin, SMALL, model.weights, kv, sentences=1, beams=W) for kv in (long, short))
+    try:
+        a.start([prompt])
+        b.start([prompt])
+        for step in range(5):  # positions 11 to 15
+            for x, y in zip(a.step(), b.step()):
+                assert np.array_equal(x, y)
+        assert short.lens.tolist() == [16] * W
+        before = b.tokens.copy(), b.scores.copy()
+        with pytest.raises(StrataError) as e:
+            b.step()
+        assert e.value.code == -3 and short.lens.tolist() == [16] * W
+        assert np.array_equal(b.tokens, before[0]) and np.array_equal(b.scores, before[1])
+        a.step()
+        b.start([prompt])  # the cache can be used again
+        a.start([prompt])
+        for x, y in zip(a.step(), b.step()):
+            assert np.array_equal(x, y)
+        hist, scores = b.search([prompt], 5)
+        assert all(len(h) == 5 for h in hist[0])
+    finally:
+        a.release()
+        b.release()
+        long.release()
+        short.release()
