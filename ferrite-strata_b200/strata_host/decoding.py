@@ -405,14 +405,36 @@ class TreeDecoder(_Decoder):
         self.prefill({r: p[:-1] for r, p in enumerate(prompts)})
         self.newest = np.array([p[-1] for p in prompts], np.int32)
 
+    def _make_room(self, count) -> None:
+        """Pages for ``count[r]`` nodes of each row; a partly filled page becomes the row's own.  As many
+        for every row as the largest tree takes, by one fork, where they fit; else each row's own."""
+        kv, rows, most = self.kv, np.arange(self.kv.rows), int(count.max())
+        if (kv.lens + most <= kv.pages_per_row * kv.page_size).all():
+            try:
+                kv.fork(rows, reserve=most)
+                return
+            except StrataError as e:
+                if e.code != abi.RESOURCE_EXHAUSTED:
+                    raise
+        kv.fork(rows, reserve=0)
+        kv.reserve(count)
+
     def step(self, drafts):
         """``drafts[r]``: (tokens, parents) of row r's drafted nodes, parents among the nodes before
-        (0: the newest token).  Returns, per row, the tokens the model's argmax accepts and the one
-        it adds: at least one."""
+        (0: the newest token), or None for a row that sits the step out.  Returns, per row, the tokens
+        the model's argmax accepts and the one it adds: at least one, none for a row that sits out.
+        Where a row or the pool has no room for its nodes, nothing changes."""
         kv, T, B = self.kv, self.nodes, self.kv.rows
         ids, parents = np.zeros((B, T), np.int32), np.zeros((B, T), np.int32)
         pos, count = np.zeros((B, T), np.int32), np.zeros(B, np.int32)
-        for r, (tokens, par) in enumerate(drafts):
+        if len(drafts) != B:
+            raise ValueError("one draft, or None, per row")
+        for r, draft in enumerate(drafts):
+            if draft is None:
+                parents[r, 0] = -1
+                pos[r] = kv.lens[r]
+                continue
+            tokens, par = draft
             n = 1 + len(tokens)
             if n > T or len(par) != len(tokens):
                 raise ValueError(f"a tree has at most {T} nodes, its first the newest token")
@@ -423,7 +445,7 @@ class TreeDecoder(_Decoder):
             for t in range(1, n):
                 pos[r, t] = pos[r, parents[r, t]] + 1
             pos[r] += kv.lens[r]
-        kv.fork(np.arange(B), reserve=T)
+        self._make_room(count)
         for b, x in ((self._ids, ids), (self._pos, pos), (self._base, kv.lens), (self._count, count),
                      (self._mask, ancestor_masks(parents))):
             b.write(np.ascontiguousarray(x))
@@ -431,6 +453,10 @@ class TreeDecoder(_Decoder):
         best = np.frombuffer(self._out.read(), np.int32).reshape(B, T)
         paths, found = [], []
         for r in range(B):
+            if not count[r]:
+                paths.append([])
+                found.append([])
+                continue
             path, got = [0], [int(best[r, 0])]
             while True:
                 nxt = next((t for t in range(path[-1] + 1, count[r])

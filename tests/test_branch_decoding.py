@@ -575,3 +575,69 @@ def test_a_beam_search_goes_to_its_rows_end(cuda, plugin, model):
         b.release()
         long.release()
         short.release()
+
+
+@pytest.mark.gpu
+def test_tree_steps_near_a_rows_end_and_rows_that_sit_out(cuda, plugin, model):
+    """A draft that fits its row is checked however many nodes the graph has; a row without a
+    draft stays as it is, at any length, and goes on later."""
+    rng = np.random.default_rng(7)
+    prompts = [[int(x) for x in rng.integers(0, 300, n)] for n in (31, 5)]
+    kv = PagedKv(plugin, pools=2 * SMALL.layers, pages=6, kv_heads=2, page_size=16, head_dim=64, rows=2,
+                 pages_per_row=2)
+    dec = TreeDecoder(plugin, SMALL, model.weights, kv, nodes=9)
+
+    def right(seq, got):
+        for t in got:
+            x = model.logits(seq)
+            assert t == int(np.argmax(x)) or _gap(x) < 0.02
+            seq.append(t)
+
+    try:
+        dec.start(prompts)
+        seqs = [list(p) for p in prompts]
+        for drafts in ([([], []), ([1, 2, 3], [0, 1, 0])], [([], []), None], [None, ([], [])]):
+            lens = kv.lens.copy()
+            found = dec.step(drafts)
+            for r, (d, got) in enumerate(zip(drafts, found)):
+                assert kv.lens[r] == lens[r] + len(got) and (d is None) == (got == [])
+                right(seqs[r], got)
+        assert kv.lens[0] == 32
+        with pytest.raises(StrataError) as e:
+            dec.step([([], []), ([], [])])  # row 0 is full
+        assert e.value.code == -3
+        lens = kv.lens.copy()
+        (none, got) = dec.step([None, ([4, 4], [0, 0])])
+        assert none == [] and kv.lens[0] == 32 and kv.lens[1] == lens[1] + len(got)
+        right(seqs[1], got)
+        assert dec.step([None, None]) == [[], []]
+    finally:
+        dec.release()
+        kv.release()
+
+
+@pytest.mark.gpu
+def test_a_tree_step_writes_no_page_that_another_row_shares(cuda, plugin, model):
+    """A row that goes back into a page it shares gets a copy, also where only its own room fits."""
+    prompt = [int(x) for x in np.random.default_rng(8).integers(0, 300, 33)]
+    kv = PagedKv(plugin, pools=2 * SMALL.layers, pages=5, kv_heads=2, page_size=16, head_dim=64, rows=2,
+                 pages_per_row=3)
+    dec = TreeDecoder(plugin, SMALL, model.weights, kv, nodes=9)
+    try:
+        for sits_out in (False, True):
+            dec.start([prompt, [1]])
+            kv.fork([0, 0], reserve=0)  # two full pages, shared
+            kv.lens[1] = 20
+            dec.newest[1] = prompt[20]
+            got = dec.step([None if sits_out else ([], []), ([7] * 8, [0] * 8)])
+            x = model.logits(prompt[:21])
+            assert got[1][0] == int(np.argmax(x)) or _gap(x) < 0.02
+            if sits_out:
+                got = dec.step([([], []), None])
+            x = model.logits(prompt)
+            assert got[0][0] == int(np.argmax(x)) or _gap(x) < 0.02
+            table = np.frombuffer(kv.table.read(), np.int32).reshape(2, 3)
+            assert table[0, 0] == table[1, 0] and table[0, 1] != table[1, 1]
+    finally:
+        dec.release()
+        kv.release()
