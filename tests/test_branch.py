@@ -445,6 +445,48 @@ def test_tree_attention_reports_a_missing_page(cuda, lib):
     t.go(torch, lib)
 
 
+class HoledTree(Tree):
+    """A paged call some of whose table entries name no page: cached positions there read as zero
+    rows (score 0 and value 0, counted in the softmax), and nodes there are attended but not stored."""
+
+    def punch(self, holes):
+        """holes: (sequence, page of the sequence, the entry put there)."""
+        self.stale(np.nan)
+        self.sound = self.table.copy()
+        for b, i, entry in holes:
+            self.table[b, i] = entry
+
+    def answer(self):
+        named, caches = self.table, (self.kc, self.vc)
+        bad = (named < 0) | (named >= self.pages)
+        # every hole a zero page of its own, behind the pool
+        self.table = named.copy()
+        self.table[bad] = self.pages + np.arange(bad.sum())
+        self.kc, self.vc = (np.concatenate([c, np.zeros((bad.sum(), *c.shape[1:]), c.dtype)]) for c in caches)
+        out, tol, kc, vc = super().answer()
+        self.table, (self.kc, self.vc) = named, caches
+        return out, tol, kc[:self.pages], vc[:self.pages]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,H,G,d,page,base,holes", [
+    (8, 4, 2, 128, 16, [200, 40], [(0, 1, -1)]),                          # inside the first tile
+    (8, 4, 2, 64, 16, [200, 140], [(0, 9, 1 << 30), (1, 0, -7)]),         # in a later tile; the first page
+    (3, 8, 1, 128, 64, [640, 250], [(0, 2, -1), (0, 3, -1), (1, 1, 10 ** 6)]),  # a whole tile
+    (5, 4, 4, 64, 128, [500, 129], [(0, 1, -1), (1, 0, -1)]),
+    (40, 8, 1, 128, 16, [390, 64], [(0, 3, -1), (0, 20, -1), (1, 3, -1)]),  # two query tiles a kv head
+    (40, 8, 1, 64, 256, [390, 600], [(0, 0, -1), (1, 2, -1)]),
+    (20, 4, 2, 128, 16, [100, 37], [(0, 7, -1), (1, 2, -1), (1, 3, 1 << 30)]),  # pages of nodes, and of both
+])
+def test_tree_attention_reads_missing_pages_as_zero_rows(cuda, lib, T, H, G, d, page, base, holes):
+    L = -(-(max(base) + T) // page) * page
+    t = HoledTree(T + d + page, 2, T, H, G, d, L, base, page=page)
+    t.punch(holes)
+    t.go(cuda, lib, status=6)
+    t.table = t.sound  # the same call with all its pages
+    t.go(cuda, lib)
+
+
 @pytest.mark.gpu
 def test_tree_attention_in_graphs_and_on_two_streams(cuda, lib):
     """A captured call replayed on new inputs, and two calls in flight at once
