@@ -207,9 +207,12 @@ int32_t strata_b200_argmax_bf16(const uint16_t *x, int64_t rows, int64_t cols,
  *    replayed at once.
  *  - `status` (null, or one I32 on the device) is set when a device-side
  *    input is wrong, and left alone otherwise: 2 a length, position or index
- *    out of range, 6 a block-table entry that names no page of the pool.
+ *    out of range, 6 a block-table entry that names no page of the pool; 4 is a
+ *    fault of the library's own (a wait inside a kernel ran out; outputs are then
+ *    incomplete).
  *  - Calls allocate nothing and may be captured into a CUDA graph.  Launches
- *    go to the current device, which must be the stream's. */
+ *    go to the current device, which must be the stream's.  What a call writes
+ *    is there for every later call on its stream, without a wait between. */
 
 /* Attention of a tree of drafted tokens over the cached prompt.  q
  * [batch * tokens, heads * head_dim]; k_new, v_new [batch * tokens,
@@ -219,13 +222,16 @@ int32_t strata_b200_argmax_bf16(const uint16_t *x, int64_t rows, int64_t cols,
  * nodes j whose bit j % 32 of word j / 32 is set in mask [batch, tokens,
  * ceil(tokens / 32)] row t (set a node's own bit to let it see itself).  out
  * [batch * tokens, heads * head_dim]; a node that sees nothing, and rows at or
- * past count, are zeros.  A sequence with base < 0, count outside 0..tokens or
- * base + count > max_len gets status 2: zeros, and nothing is appended.
- * Positions on missing pages get status 6 and read as zero rows.  tokens <=
- * 1024, head_dim 64 or 128, at most 128 query heads per kv head, pointers
- * 16-byte aligned; a call whose 128-position tiles over all sequences and kv
- * heads could pass 2^31 is refused.  Two sequences must not append to the same
- * page. */
+ * past count, are zeros.  Scores, softmax sums and accumulators are f32; each
+ * probability is rounded to bf16 (by at most 2^-8 of it) for its product with v,
+ * as in the library's other attention, so an output is within
+ * 2^-8 sum_p(w_p |v_p|) + 2^-8 |o| and 32-bit rounding.  A sequence with
+ * base < 0, count outside 0..tokens or base + count > max_len gets status 2:
+ * zeros, and nothing is appended.  Positions on missing pages get status 6 and
+ * read as zero rows.  tokens <= 1024, head_dim 64 or 128, at most 128 query
+ * heads per kv head, pointers 16-byte aligned; a call whose 128-position tiles
+ * over all sequences and kv heads could pass 2^31 is refused.  Two sequences
+ * must not append to the same page. */
 uint64_t strata_b200_tree_attention_workspace_bytes(int64_t tokens,
                                                     int64_t heads,
                                                     int64_t kv_heads,
@@ -240,9 +246,10 @@ int32_t strata_b200_tree_attention_bf16(
 
 /* A beam step's selection.  logits [batch * beams, vocab]; scores
  * [batch * beams], the beams' accumulated log probabilities (-inf or NaN: an
- * empty beam); done [batch * beams] (may be null), non-zero for a beam that has
- * ended.  A live beam w offers score + log_softmax(logits)[v] for every v (a NaN
- * logit counts as -inf); an ended one offers its unchanged score with token
+ * empty beam, which offers nothing); done [batch * beams] (may be null),
+ * non-zero for a beam that has ended.  A live beam w offers score + log_softmax(logits)[v] for every v (a NaN
+ * logit counts as -inf; +inf logits share their row's probability equally and
+ * the others get none); an ended one offers its unchanged score with token
  * eos.  Writes the `keep` best of every batch entry, best first, ties to the
  * lowest w * vocab + v: out_scores, out_parent (the row b * beams + w),
  * out_token and out_done (the parent had ended, or the token is eos), each
@@ -250,7 +257,10 @@ int32_t strata_b200_tree_attention_bf16(
  * eos -1: no token ends a beam (an ended beam's token is then -1).  keep <=
  * 64, beams <= 1024, batch * beams <= 65535, vocab <= 2^30.  Scores are added
  * and compared in f64 and rounded once; the softmax's terms are f32, and the
- * logarithm of their sum is within 2^-20. */
+ * logarithm of their sum is within 2^-20.  Each beam enters with its `keep`
+ * largest logits (the lowest ids on ties): where two different logits of a beam
+ * are so close beside its score that f64 gives both the same score, the larger
+ * logit may be kept and not the lower id. */
 uint64_t strata_b200_beam_select_workspace_bytes(int64_t batch, int64_t beams,
                                                  int64_t vocab, int64_t keep);
 int32_t strata_b200_beam_select_bf16(
