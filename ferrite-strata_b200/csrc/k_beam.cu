@@ -24,7 +24,7 @@
 // a list of its own, against 37, for 512 rows of 128001 bf16, keep 32); a ring of
 // asynchronous copies to shared memory cost more in resident blocks than it hid
 // (54 us).  Without the last part the pass takes 28 us, 4.7 TB/s.  With the joining
-// kernel, about 7 us, the call takes 44 us; 4 rows of 32000 f32 take 10 us, which is
+// kernel, about 7 us, the call takes 46 us; 4 rows of 32000 f32 take 11 us, which is
 // the latency of two kernels.
 //
 // Scores are compared in 64 bits: two beams' candidates can lie closer than

@@ -7,11 +7,11 @@
 // All three move whole 16-byte pieces and compute nothing on them, so they
 // are exact in any element type; what bounds them is HBM (every moved byte is
 // read once and written once) or, for a few rows, latency.  Measured, device time
-// back to back in a graph: accepting one sequence's path in 64 caches 3.1 us (the
-// host's launch takes 9), 32 paths of up to 33 nodes in 160 pools 14.7 us; forking 4
-// rows of 64 pools 9.9 us, most of it the plan's chain of dependent reads; 128 rows of
-// 32 pools 46 us, the copies alone (220 MB) 39 us with nothing cached, 5.6 TB/s;
-// compacting 3000 pages of 32 pools 240 us, the copies 236 us, 6.1 TB/s.
+// back to back in a graph: accepting one sequence's path in 64 caches 2.8 us (the
+// host's launch takes 9), 32 paths of up to 33 nodes in 160 pools 17.5 us; forking 4
+// rows of 64 pools 11.5 us, most of it the plan's chain of dependent reads; 128 rows of
+// 32 pools 47 us, the copies alone (220 MB) 41 us with nothing cached, 5.4 TB/s;
+// compacting 3000 pages of 32 pools 241 us, the copies 238 us, 6.0 TB/s.
 //
 // What these kernels write, the decode attention may read before its wait (rows
 // below a position, the block table, positions).  So no later kernel may start

@@ -45,7 +45,10 @@
 // when a score exceeds the reference by more than 8, so probabilities stay
 // below 2^8.  The two threads of a row agree by one barrier vote per tile that
 // nothing moves; only when something does they exchange their maxima.  P is
-// rounded to bf16 for the second product; reference, sum and O are f32.
+// rounded to bf16 for the second product, whose operands have to be of V's type
+// (f32 terms would take a second product for what the rounding leaves); each
+// probability is then off by at most 2^-8, which for values without a common sign
+// adds as much error as rounding the output does.  Reference, sum and O are f32.
 //
 // Masked places.  A masked score becomes -inf whatever it was.  0 * NaN must
 // not reach O either: V rows at or past a tile's end are zeroed in shared
