@@ -303,8 +303,9 @@ int32_t strata_b200_kv_accept(
  * input) and report I32 [4]: error, pages copied, pages newly reserved, pages
  * left free.  Errors: 2 a parent or length out of range (or len + reserve past
  * the row), 3 refs below the table's references, 5 too few free pages (report
- * [3] is how many more are needed), 6 a needed entry that names no page; the
- * outputs are then copies of the inputs and the pools are not touched.
+ * [3] is how many more are needed), 6 a needed entry that names no page; where
+ * several hold, 6 goes before 3 before 2 before 5.  The outputs are then copies
+ * of the inputs and the pools are not touched.
  * rows <= 65536, rows * pages_per_seq < 2^31 - 8192; a call with no rows writes
  * nothing. */
 uint64_t strata_b200_kv_fork_workspace_bytes(int64_t rows,
