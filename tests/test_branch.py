@@ -1112,9 +1112,10 @@ class DecodeAttention:
 
 
 def _back_to_back(torch, first, then, restore):
-    """Bits of `then()`'s outputs where the GPU is waited for between the two, and without, eagerly and in a graph."""
-    def go(between):
-        restore()
+    """Bits of `then()`'s outputs where the GPU is waited for between the two, and without, eagerly and
+    in a graph; two sets of inputs in turn, so that what one left in a cache is wrong for the other."""
+    def go(between, which):
+        restore(which)
         torch.cuda.synchronize()
         first()
         if between:
@@ -1123,23 +1124,23 @@ def _back_to_back(torch, first, then, restore):
         torch.cuda.synchronize()
         return [o.view(torch.int16).clone() for o in outs]
 
-    want = go(True)
-    for _ in range(10):
-        assert all(torch.equal(a, b) for a, b in zip(want, go(False)))
+    want = [go(True, 0), go(True, 1)]
+    assert not any(torch.equal(a, b) for a, b in zip(*want))
+    for i in range(12):
+        assert all(torch.equal(a, b) for a, b in zip(want[i % 2], go(False, i % 2)))
     s = torch.cuda.Stream()
     with torch.cuda.stream(s):
-        restore()
+        restore(0)
         s.synchronize()
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g, stream=s):
             first()
             outs = then()
-        for _ in range(5):
-            restore()
+        for i in range(6):
+            restore(i % 2)
             g.replay()
             s.synchronize()
-            assert all(torch.equal(a, b.view(torch.int16)) for a, b in zip(want, outs))
-    return want
+            assert all(torch.equal(a, b.view(torch.int16)) for a, b in zip(want[i % 2], outs))
 
 
 @pytest.mark.gpu
@@ -1154,10 +1155,12 @@ def test_decode_attention_right_behind_an_accept(cuda, lib, G, d):
     gen = torch.Generator("cuda").manual_seed(1)
     init = torch.randn((2 * layers, B, G, L, d), device="cuda", generator=gen, dtype=torch.bfloat16)
     caches = init.clone()
-    base = D(rng.integers(0, L - 2 * width, B).astype(np.int32))
-    path = D(np.stack([np.sort(rng.choice(2 * width, width, replace=False)) for _ in range(B)]).astype(np.int32))
+    bases = [D(rng.integers(0, L - 2 * width, B).astype(np.int32)) for _ in range(2)]
+    paths = [D(np.stack([np.sort(rng.choice(2 * width, width, replace=False)) for _ in range(B)]).astype(np.int32))
+             for _ in range(2)]
+    base, path = torch.empty_like(bases[0]), torch.empty_like(paths[0])
     n = D(np.full(B, width, np.int32))
-    pos = base + width  # the next token's position
+    pos = torch.empty_like(base)
     attend = DecodeAttention(torch, lib, B, H, G, d, L)
     outs = [torch.empty(B, H * d, dtype=torch.bfloat16, device="cuda") for _ in range(layers)]
 
@@ -1170,7 +1173,13 @@ def test_decode_attention_right_behind_an_accept(cuda, lib, G, d):
             attend(caches[2 * i], caches[2 * i + 1], pos, outs[i])
         return outs
 
-    _back_to_back(torch, accept, step, lambda: caches.copy_(init))
+    def restore(which):
+        caches.copy_(init)
+        base.copy_(bases[which])
+        path.copy_(paths[which])
+        pos.copy_(bases[which] + width)  # the next token's position
+
+    _back_to_back(torch, accept, step, restore)
 
 
 @pytest.mark.gpu
@@ -1187,9 +1196,13 @@ def test_decode_attention_right_behind_tree_attention(cuda, lib, T, H, G, d):
     attend = DecodeAttention(torch, lib, B, H, G, d, L)
     out = torch.empty(B, H * d, dtype=torch.bfloat16, device="cuda")
 
-    def restore():
-        s["kc"].copy_(init[0])
-        s["vc"].copy_(init[1])
+    new = [(s["k"].clone(), s["v"].clone()), (s["k"].flip(0).clone(), s["v"].flip(0).clone())]
+
+    def restore(which):
+        for c, x in zip((s["kc"], s["vc"]), init):
+            c.copy_(x)
+        for c, x in zip((s["k"], s["v"]), new[which]):
+            c.copy_(x)
 
     def step():
         attend(s["kc"], s["vc"], pos, out)

@@ -407,7 +407,13 @@ def test_a_step_right_behind_a_page_operation(cuda, plugin, op):
     refs[ids[:at]] = 1
     init = torch.randn((pools, pages, G, ps, d), device="cuda", dtype=torch.bfloat16)
     pool = init.clone()
-    ti, li, ri, pa = dev(table), dev(lens), dev(refs), dev(rng.integers(0, R, R).astype(np.int32))
+    ti, li, ri, pa = dev(table), dev(lens), dev(refs), i32(R)
+    # two forks, or two placings of the same pages, in turn: what one left in a cache is wrong for the other
+    parents = [dev(rng.integers(0, R, R).astype(np.int32)) for _ in range(2)]
+    tables, counts = [ti.clone()], [ri.clone()]
+    other = rng.permutation(pages).astype(np.int32)
+    tables.append(dev(np.where(table >= 0, other[table], -1)))
+    counts.append(dev(refs[np.argsort(other)]))
     to, lo, ro, remap, report = i32(R, per), i32(R), i32(pages), i32(pages), i32(4)
     n_pools = 0 if "alone" in op else pools
     ptrs = (ctypes.c_void_p * pools)(*[p.data_ptr() for p in pool])
@@ -420,7 +426,7 @@ def test_a_step_right_behind_a_page_operation(cuda, plugin, op):
     lib.strata_b200_kv_fork.argtypes = [P] + [I64] * 5 + [P] * 4 + [I64] * 3 + [P] * 6
     lib.strata_b200_kv_compact.argtypes = [P] + [I64] * 5 + [P] * 2 + [I64] * 2 + [P] * 6
 
-    def page_op():
+    def page_op(ti=ti, ri=ri, pa=pa):
         if op == "compact":
             return lib.strata_b200_kv_compact(ptrs, n_pools, 2 * d, G, ps, pages, ti.data_ptr(), ri.data_ptr(), R, per,
                                               to.data_ptr(), ro.data_ptr(), remap.data_ptr(), report.data_ptr(),
@@ -443,10 +449,12 @@ def test_a_step_right_behind_a_page_operation(cuda, plugin, op):
              outs[0]: out}
     bufs = {i: plugin.wrap(t.data_ptr(), t.numel() * t.element_size()) for i, t in where.items()}
 
-    def go(wait):
+    def go(wait, which):
         pool.copy_(init)
-        for x in (to, lo):
-            x.fill_(0)
+        pa.copy_(parents[which])
+        if op == "compact":
+            ti.copy_(tables[which])
+            ri.copy_(counts[which])
         torch.cuda.synchronize()
         exe = plugin.compile(g)  # a new one: its first run is not a captured one
         run = exe.bind({i: Device(x) for i, x in bufs.items()})
@@ -462,10 +470,39 @@ def test_a_step_right_behind_a_page_operation(cuda, plugin, op):
             run.release()
             exe.free()
 
-    want = go(True)
-    assert want.any()
-    for _ in range(10):
-        assert torch.equal(want, go(False))
+    want = [go(True, 0), go(True, 1)]
+    assert not torch.equal(*want)
+    for i in range(12):
+        assert torch.equal(want[i % 2], go(False, i % 2))
+
+    def chain(wait):  # operation, step, the other operation, step, ... with nothing else between
+        pool.copy_(init)
+        sinks = [torch.empty_like(out) for _ in range(6)]
+        wrapped = [plugin.wrap(x.data_ptr(), x.numel() * 2) for x in sinks]
+        exes = [plugin.compile(g) for _ in sinks]
+        runs = [e.bind({**{i: Device(x) for i, x in bufs.items()}, outs[0]: Device(w)}) for e, w in zip(exes, wrapped)]
+        torch.cuda.synchronize()
+        try:
+            for i, run in enumerate(runs):
+                assert page_op(tables[i % 2], counts[i % 2], parents[i % 2]) == 0
+                if wait:
+                    torch.cuda.synchronize()
+                run.run_async()
+                if wait:
+                    plugin.synchronize()
+            plugin.synchronize()
+            return torch.stack(sinks).view(torch.int16)
+        finally:
+            for x in (*runs, *wrapped):
+                x.release()
+            for e in exes:
+                e.free()
+
+    if op != "compact":  # the first page set serves both forks
+        tables[1], counts[1] = tables[0], counts[0]
+    steps = chain(True)
+    for _ in range(4):
+        assert torch.equal(steps, chain(False))
     for x in bufs.values():
         x.release()
 
